@@ -19,6 +19,8 @@ EXPORTS = (
     "brisk_hip_last_error", "brisk_hip_abi_version", "brisk_hip_device_count", "brisk_hip_packed_bytes", "brisk_hip_pack",
     "brisk_hip_quantize_q8_0", "brisk_hip_quantize_q8_k", "brisk_hip_matvec", "brisk_hip_matmul", "brisk_hip_matmul_noalloc", "brisk_hip_gemv", "brisk_hip_expf", "brisk_hip_tanhf", "brisk_hip_log1pf",
     "brisk_hip_div_selftest", "brisk_hip_mfma_rate",
+    "brisk_hip_kv_bytes", "brisk_hip_qk_norm_rope", "brisk_hip_kv_append", "brisk_hip_kv_read",
+    "brisk_hip_paged_attention_bytes", "brisk_hip_paged_attention",
     "brisk_hip_session_estimate", "brisk_hip_device_memory", "brisk_hip_session_create", "brisk_hip_session_destroy", "brisk_hip_session_eval", "brisk_hip_session_eval_all",
     "brisk_hip_session_eval_greedy", "brisk_hip_session_generate", "brisk_hip_session_decode", "brisk_hip_session_rollback",
     "brisk_hip_session_position", "brisk_hip_session_max_context", "brisk_hip_session_kv_cache",
@@ -47,6 +49,27 @@ class HipTensor(C.Structure):
 
 class HipMemory(C.Structure):
     _fields_ = [("weights", C.c_size_t), ("cache", C.c_size_t), ("scratch", C.c_size_t), ("total", C.c_size_t)]
+
+
+class HipHeads(C.Structure):
+    """A [rows][heads][head_dim] device tensor (brisk_hip_heads); strides in values."""
+    _fields_ = [("data", C.c_void_p), ("type", C.c_int), ("row_stride", C.c_size_t), ("head_stride", C.c_size_t)]
+
+
+class HipRope(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("positions", C.c_uint32), ("dims", C.c_uint32), ("neox", C.c_int32)]
+
+
+class HipKv(C.Structure):
+    """A paged key/value cache (brisk_hip_kv)."""
+    _fields_ = [("data", C.c_void_p), ("type", C.c_int), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("page_tokens", C.c_uint32), ("pages", C.c_uint32)]
+
+
+class HipBatch(C.Structure):
+    """Sequences, their rows and their pages (brisk_hip_batch)."""
+    _fields_ = [("row_start", C.c_void_p), ("lengths", C.c_void_p), ("page_table", C.c_void_p), ("seqs", C.c_uint32),
+                ("rows", C.c_uint32), ("page_stride", C.c_uint32), ("max_rows", C.c_uint32), ("max_length", C.c_uint32)]
 
 
 class BriskHipError(RuntimeError):
@@ -82,6 +105,15 @@ def load():
     L.brisk_hip_log1pf.argtypes = [_vp, _vp, _sz, _vp]
     L.brisk_hip_div_selftest.argtypes = [C.POINTER(C.c_ulonglong)]
     L.brisk_hip_mfma_rate.argtypes = [_i, C.POINTER(C.c_double)]
+    heads, rope, kv, batch = C.POINTER(HipHeads), C.POINTER(HipRope), C.POINTER(HipKv), C.POINTER(HipBatch)
+    L.brisk_hip_kv_bytes.argtypes = [kv]
+    L.brisk_hip_kv_bytes.restype = _sz
+    L.brisk_hip_qk_norm_rope.argtypes = [heads, heads, _sz, C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _f, rope, _vp, heads, heads, _vp]
+    L.brisk_hip_kv_append.argtypes = [kv, batch, heads, heads, _vp, _f, rope, _vp]
+    L.brisk_hip_kv_read.argtypes = [kv, batch, heads, heads, _vp]
+    L.brisk_hip_paged_attention_bytes.argtypes = [kv, batch, C.c_uint32]
+    L.brisk_hip_paged_attention_bytes.restype = _sz
+    L.brisk_hip_paged_attention.argtypes = [kv, batch, heads, C.c_uint32, _f, C.c_uint32, heads, _vp, _sz, _vp]
     L.brisk_hip_session_estimate.argtypes = [C.POINTER(HipConfig), C.POINTER(HipTensor), _sz, _sz, C.POINTER(HipMemory)]
     L.brisk_hip_device_memory.argtypes = [_i, C.POINTER(_sz), C.POINTER(_sz)]
     L.brisk_hip_session_create.argtypes = [C.POINTER(HipConfig), C.POINTER(HipTensor), _sz, _sz, _i, C.POINTER(_vp)]

@@ -1,11 +1,13 @@
 // The extern "C" surface declared in include/brisk_hip.h.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <exception>
 #include <mutex>
 #include <new>
 #include <string>
 
+#include "paged.h"
 #include "prefill.h"
 #include "session.h"
 
@@ -88,6 +90,73 @@ void* noalloc_scratch() {
         ptrs[dev] = ptr;
     }
     return ptrs[dev];
+}
+
+// ---- the paged cache's arguments
+
+[[noreturn]] void bad(const std::string& what) { throw bh::Error(BRISK_HIP_EINVAL, "kernels: " + what); }
+
+bh::HeadRows head_rows(const brisk_hip_heads* x, const char* name) {
+    if (x == nullptr || x->data == nullptr) bad(std::string("null ") + name);
+    if (x->type != BRISK_HIP_F32 && x->type != BRISK_HIP_F16 && x->type != BRISK_HIP_BF16)
+        bad(std::string(name) + " must be F32, F16 or BF16");
+    const size_t size = x->type == BRISK_HIP_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(x->data) % size != 0) bad(std::string(name) + " is not aligned to its type");
+    constexpr size_t most = size_t{1} << 40;
+    if (x->row_stride > most || x->head_stride > most) bad(std::string(name) + " has a stride that is too large");
+    return {x->data, x->type, static_cast<int64_t>(x->row_stride), static_cast<int64_t>(x->head_stride)};
+}
+
+// A tensor that is written: its rows and heads must not overlap.
+bh::HeadRows written_rows(const brisk_hip_heads* x, const char* name, size_t rows, uint32_t heads, uint32_t head_dim) {
+    const bh::HeadRows r = head_rows(x, name);
+    const size_t a = x->row_stride, b = x->head_stride;
+    const bool by_row = (heads == 1 || b >= head_dim) && (rows == 1 || a >= (heads - 1) * b + head_dim);
+    const bool by_head = (rows == 1 || a >= head_dim) && (heads == 1 || b >= (rows - 1) * a + head_dim);
+    if (!by_row && !by_head) bad(std::string(name) + " has rows or heads that overlap");
+    return r;
+}
+
+bh::RopeTable rope_table(const brisk_hip_rope* rope, uint32_t head_dim) {
+    if (rope == nullptr) return {nullptr, 0, 0, 0};
+    if (rope->table == nullptr || rope->positions == 0) bad("empty rotation table");
+    if (reinterpret_cast<uintptr_t>(rope->table) % 4 != 0) bad("the rotation table is not aligned to its type");
+    if (rope->dims == 0 || rope->dims % 2 != 0 || rope->dims > head_dim) bad("the rotated dimensions must be even and at most the head size");
+    if (rope->neox != 1 && rope->neox != 2) bad("neox must be 1 or 2");
+    return {rope->table, rope->positions, rope->dims, rope->neox == 1};
+}
+
+bool kv_shape_taken(const brisk_hip_kv* kv) {
+    const uint32_t d = kv->head_dim, t = kv->page_tokens;
+    return (kv->type == BRISK_HIP_F16 || kv->type == BRISK_HIP_Q4_0) && (d == 64 || d == 96 || d == 128 || d == 256 || d == 512) &&
+           t >= bh::kTileTokens && t <= bh::kMaxPageTokens && (t & (t - 1)) == 0 && kv->kv_heads >= 1 && kv->kv_heads <= 1024 &&
+           kv->pages >= 1 && kv->pages <= 0x7FFFFFFFu;
+}
+
+bh::PagedKv paged_kv(const brisk_hip_kv* kv, bool data) {
+    if (kv == nullptr) bad("null cache");
+    if (!kv_shape_taken(kv))
+        bad("a cache is F16 or Q4_0, of 1 to 1024 heads of 64, 96, 128, 256 or 512 values and pages of a power of two of 16 to 1024 positions");
+    if (data && kv->data == nullptr) bad("null cache");
+    if (data && reinterpret_cast<uintptr_t>(kv->data) % 16 != 0) bad("the cache is not 16-byte aligned");
+    return {static_cast<uint8_t*>(kv->data), kv->type == BRISK_HIP_Q4_0, kv->kv_heads, kv->head_dim, kv->page_tokens, kv->pages,
+            static_cast<uint32_t>(__builtin_ctz(kv->page_tokens))};
+}
+
+bh::PagedBatch paged_batch(const brisk_hip_batch* b, bool data) {
+    if (b == nullptr) bad("null batch");
+    if (b->rows > 0x7FFFFFFFu || b->seqs > 0x7FFFFFFEu) bad("too many rows or sequences");
+    if (data && b->seqs != 0 && (b->row_start == nullptr || b->lengths == nullptr)) bad("null row starts or lengths");
+    if (data && b->seqs != 0 && b->page_stride != 0 && b->page_table == nullptr) bad("null page table");
+    if (reinterpret_cast<uintptr_t>(b->row_start) % 4 != 0 || reinterpret_cast<uintptr_t>(b->lengths) % 4 != 0 ||
+        reinterpret_cast<uintptr_t>(b->page_table) % 4 != 0)
+        bad("a batch array is not aligned to its type");
+    return {b->row_start, b->lengths, b->page_table, b->seqs, b->rows, b->page_stride, b->max_rows, b->max_length};
+}
+
+uint32_t head_group(uint32_t heads, const bh::PagedKv& kv) {
+    if (heads == 0 || heads > 65536 || heads % kv.kv_heads != 0) bad("the query heads must be a multiple of the key/value heads");
+    return heads / kv.kv_heads;
 }
 
 }  // namespace
@@ -284,6 +353,110 @@ int brisk_hip_mfma_rate(int shape, double* int8_tops) {
         const double per_iter = shape == 0 ? 8.0 * 16 * 16 * 64 : 4.0 * 32 * 32 * 32;
         const double ops = static_cast<double>(blocks) * (bh::kThreads / 64) * iters * per_iter * 2;
         *int8_tops = ops / (ms * 1e-3) / 1e12;
+    });
+}
+
+size_t brisk_hip_kv_bytes(const brisk_hip_kv* kv) {
+    if (kv == nullptr || !kv_shape_taken(kv)) return 0;
+    return static_cast<size_t>(kv->pages) * kv->kv_heads * (kv->page_tokens / bh::kTileTokens) *
+           bh::tile_bytes(kv->type == BRISK_HIP_Q4_0, kv->head_dim / 32);
+}
+
+int brisk_hip_qk_norm_rope(const brisk_hip_heads* q, const brisk_hip_heads* k, size_t n, uint32_t heads, uint32_t kv_heads,
+                           uint32_t head_dim, const float* q_norm, const float* k_norm, float eps, const brisk_hip_rope* rope,
+                           const int32_t* positions, const brisk_hip_heads* q_out, const brisk_hip_heads* k_out, void* stream) {
+    return guarded([&] {
+        if (head_dim == 0 || head_dim % 8 != 0 || head_dim > bh::kMaxPagedHead) bad("the head size must be a multiple of 8, at most 512");
+        if (n > 0x7FFFFFFFu) bad("too many rows");
+        if (heads == 0 || heads > 65536 || (k != nullptr && (kv_heads == 0 || kv_heads > 65536))) bad("bad head count");
+        if ((k == nullptr) != (k_out == nullptr)) bad("keys need an output, and the other way round");
+        if (!(eps >= 0)) bad("eps must not be negative");
+        bh::NormRopeArgs a{};
+        a.rope = rope_table(rope, head_dim);
+        if (rope != nullptr && n != 0 && positions == nullptr) bad("null positions");
+        if (reinterpret_cast<uintptr_t>(positions) % 4 != 0) bad("the positions are not aligned to their type");
+        if (n == 0) return;
+        a.x[0] = head_rows(q, "queries");
+        a.y[0] = written_rows(q_out, "query output", n, heads, head_dim);
+        if (k != nullptr) {
+            a.x[1] = head_rows(k, "keys");
+            a.y[1] = written_rows(k_out, "key output", n, kv_heads, head_dim);
+        }
+        a.w[0] = q_norm;
+        a.w[1] = k_norm;
+        a.heads[0] = heads;
+        a.heads[1] = kv_heads;
+        a.head_dim = head_dim;
+        a.n = n;
+        a.eps = eps;
+        a.positions = positions;
+        hip_check(bh::launch_norm_rope(a, static_cast<hipStream_t>(stream)), "qk_norm_rope");
+    });
+}
+
+int brisk_hip_kv_append(const brisk_hip_kv* kv, const brisk_hip_batch* batch, const brisk_hip_heads* k, const brisk_hip_heads* v,
+                        const float* k_norm, float eps, const brisk_hip_rope* rope, void* stream) {
+    return guarded([&] {
+        bh::AppendArgs a{};
+        a.kv = paged_kv(kv, true);
+        a.b = paged_batch(batch, true);
+        a.rope = rope_table(rope, a.kv.head_dim);
+        if (!(eps >= 0)) bad("eps must not be negative");
+        if (a.b.rows == 0 || a.b.seqs == 0) return;
+        a.k = head_rows(k, "keys");
+        a.v = head_rows(v, "values");
+        a.w = k_norm;
+        a.eps = eps;
+        hip_check(bh::launch_kv_append(a, static_cast<hipStream_t>(stream)), "kv_append");
+    });
+}
+
+int brisk_hip_kv_read(const brisk_hip_kv* kv, const brisk_hip_batch* batch, const brisk_hip_heads* k, const brisk_hip_heads* v,
+                      void* stream) {
+    return guarded([&] {
+        bh::ReadArgs a{};
+        a.kv = paged_kv(kv, true);
+        a.b = paged_batch(batch, true);
+        if (a.b.rows == 0 || a.b.seqs == 0) return;
+        if (k != nullptr) a.k = written_rows(k, "keys", a.b.rows, a.kv.kv_heads, a.kv.head_dim);
+        if (v != nullptr) a.v = written_rows(v, "values", a.b.rows, a.kv.kv_heads, a.kv.head_dim);
+        if (k == nullptr && v == nullptr) return;
+        hip_check(bh::launch_kv_read(a, static_cast<hipStream_t>(stream)), "kv_read");
+    });
+}
+
+size_t brisk_hip_paged_attention_bytes(const brisk_hip_kv* kv, const brisk_hip_batch* batch, uint32_t heads) {
+    size_t bytes = 0;
+    (void)guarded([&] {
+        const bh::PagedKv c = paged_kv(kv, false);
+        const bh::PagedBatch b = paged_batch(batch, false);
+        head_group(heads, c);
+        if (b.rows != 0 && b.seqs != 0) bytes = bh::paged_workspace(c, b, heads);
+    });
+    return bytes;
+}
+
+int brisk_hip_paged_attention(const brisk_hip_kv* kv, const brisk_hip_batch* batch, const brisk_hip_heads* q, uint32_t heads, float scale,
+                              uint32_t window, const brisk_hip_heads* out, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        bh::PagedAttnArgs a{};
+        a.kv = paged_kv(kv, true);
+        a.b = paged_batch(batch, true);
+        a.group = head_group(heads, a.kv);
+        if (!std::isfinite(scale)) bad("the score scale must be finite");
+        if (a.b.rows == 0 || a.b.seqs == 0) return;
+        a.heads = heads;
+        a.q = head_rows(q, "queries");
+        a.out = written_rows(out, "output", a.b.rows, heads, a.kv.head_dim);
+        a.scale = scale;
+        a.window = window;
+        const size_t need = bh::paged_workspace(a.kv, a.b, heads);
+        if (need > workspace_bytes || (need != 0 && workspace == nullptr))
+            bad("the attention needs " + std::to_string(need) + " bytes of workspace, and has " + std::to_string(workspace_bytes));
+        if (need != 0 && reinterpret_cast<uintptr_t>(workspace) % 16 != 0) bad("the workspace is not 16-byte aligned");
+        a.splits = bh::paged_splits(a.kv, a.b, heads);
+        a.part = static_cast<float*>(workspace);
+        hip_check(bh::launch_paged_attention(a, static_cast<hipStream_t>(stream)), "paged_attention");
     });
 }
 

@@ -1,0 +1,108 @@
+// Device helpers of the paged-cache kernels: rows of any type, and values of a tile.
+#pragma once
+
+#include "paged.h"
+
+namespace bh {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint32_t word2v __attribute__((ext_vector_type(2)));
+typedef uint32_t word4v __attribute__((ext_vector_type(4)));
+
+__device__ inline char* row_ptr(const HeadRows& x, int64_t row, int64_t head) {
+    return static_cast<char*>(x.data) + (row * x.row + head * x.head) * (x.type == kTypeF32 ? 4 : 2);
+}
+
+__device__ inline float from_bf16(uint32_t b) { return __builtin_bit_cast(float, b << 16); }
+__device__ inline float from_half(uint32_t h) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h))); }
+__device__ inline uint32_t to_half(float x) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x)); }
+// Round to nearest, ties to even; a NaN stays one.
+__device__ inline uint32_t to_bf16(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    if (x != x) return u >> 16 | 0x40;
+    return (u + 0x7FFF + (u >> 16 & 1)) >> 16;
+}
+__device__ inline uint32_t pack_half(float lo, float hi) { return to_half(lo) | to_half(hi) << 16; }
+
+__device__ inline float load1(const void* head, int type, int d) {
+    if (type == kTypeF32) return static_cast<const float*>(head)[d];
+    const uint32_t u = static_cast<const uint16_t*>(head)[d];
+    return type == kTypeF16 ? from_half(u) : from_bf16(u);
+}
+
+__device__ inline void load8(const void* head, int type, bool vec, int d, float (&x)[8]) {
+    if (!vec) {
+        for (int j = 0; j < 8; ++j) x[j] = load1(head, type, d + j);
+        return;
+    }
+    if (type == kTypeF32) {
+        const float4v *p = reinterpret_cast<const float4v*>(static_cast<const float*>(head) + d), a = p[0], b = p[1];
+        for (int j = 0; j < 4; ++j) {
+            x[j] = a[j];
+            x[4 + j] = b[j];
+        }
+        return;
+    }
+    const word4v w = *reinterpret_cast<const word4v*>(static_cast<const uint16_t*>(head) + d);
+    for (int j = 0; j < 4; ++j) {
+        x[2 * j] = type == kTypeF16 ? from_half(w[j] & 0xFFFF) : from_bf16(w[j] & 0xFFFF);
+        x[2 * j + 1] = type == kTypeF16 ? from_half(w[j] >> 16) : from_bf16(w[j] >> 16);
+    }
+}
+
+__device__ inline void store8(void* head, int type, bool vec, int d, const float (&x)[8]) {
+    if (type == kTypeF32) {
+        float* p = static_cast<float*>(head) + d;
+        if (vec) {
+            *reinterpret_cast<float4v*>(p) = float4v{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<float4v*>(p + 4) = float4v{x[4], x[5], x[6], x[7]};
+        } else {
+            for (int j = 0; j < 8; ++j) p[j] = x[j];
+        }
+        return;
+    }
+    uint32_t u[8];
+    for (int j = 0; j < 8; ++j) u[j] = type == kTypeF16 ? to_half(x[j]) : to_bf16(x[j]);
+    uint16_t* p = static_cast<uint16_t*>(head) + d;
+    if (vec) {
+        *reinterpret_cast<word4v*>(p) = word4v{u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16};
+    } else {
+        for (int j = 0; j < 8; ++j) p[j] = static_cast<uint16_t>(u[j]);
+    }
+}
+
+// Eight values of a position of a tile, from dimension d (a multiple of 8) on.
+__device__ inline void read8(const uint8_t* tile, bool q4, uint32_t nb, bool value, uint32_t token, uint32_t d, float (&x)[8]) {
+    if (!q4) {
+        uint32_t w[4];
+        if (!value) {
+            const word4v v = *reinterpret_cast<const word4v*>(tile + key_offset(false, nb, token, d));
+            for (int j = 0; j < 4; ++j) w[j] = v[j];
+        } else {
+            for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint32_t*>(tile + value_offset(false, nb, token, d + 2 * j));
+        }
+        for (int j = 0; j < 4; ++j) {
+            x[2 * j] = from_half(w[j] & 0xFFFF);
+            x[2 * j + 1] = from_half(w[j] >> 16);
+        }
+        return;
+    }
+    const float s = from_half(*reinterpret_cast<const uint16_t*>(tile + scale_offset(nb, value, token, d / 32)));
+    if (!value) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + key_offset(true, nb, token, d));
+        for (int m = 0; m < 4; ++m) {
+            x[2 * m] = (static_cast<float>(w >> (4 * m) & 15) - 8) * s;
+            x[2 * m + 1] = (static_cast<float>(w >> (4 * m + 16) & 15) - 8) * s;
+        }
+    } else {
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t c = tile[value_offset(true, nb, token, d + 2 * j)];
+            x[2 * j] = (static_cast<float>(c & 15) - 8) * s;
+            x[2 * j + 1] = (static_cast<float>(c >> 4) - 8) * s;
+        }
+    }
+}
+
+}  // namespace bh

@@ -41,9 +41,11 @@ enum {
     BRISK_HIP_ENOMEM = -4     /* device allocation failed */
 };
 
-/* Tensor types: the ggml numbers a GGUF file uses (src/gguf.h:22-27). */
+/* Tensor types: the ggml numbers a GGUF file uses (src/gguf.h:22-27).  F16 and BF16
+ * are types of the paged cache and of its rows only, not of weights. */
 enum {
     BRISK_HIP_F32 = 0,
+    BRISK_HIP_F16 = 1,
     BRISK_HIP_Q4_0 = 2,
     BRISK_HIP_Q4_1 = 3,
     BRISK_HIP_Q5_0 = 6,
@@ -51,6 +53,7 @@ enum {
     BRISK_HIP_Q4_K = 12,
     BRISK_HIP_Q5_K = 13,
     BRISK_HIP_Q6_K = 14,
+    BRISK_HIP_BF16 = 30,
     BRISK_HIP_TQ2_0 = 35
 };
 
@@ -216,6 +219,121 @@ int brisk_hip_div_selftest(unsigned long long* mismatches);
  * GEMMs' MFMA fraction is read against.  Measurement support; no counterpart
  * in the reference. */
 int brisk_hip_mfma_rate(int shape, double* int8_tops);
+
+/* ------------------------------------------------------- paged cache, kernel level
+ *
+ * A key/value cache in pages for several sequences, and what runs between the
+ * projections (brisk_hip_matmul) and the output projection's quantisation.  No
+ * counterpart in the reference, which serves one sequence from one contiguous
+ * fp16 cache (src/model.cpp:984-991).
+ *
+ * All pointers are device memory of the current device, and `stream` is one of
+ * its streams; no call allocates, synchronises or keeps anything, so every
+ * call can be captured in a HIP graph.  Calls that touch the same pages, outputs or
+ * workspace are ordered by the caller (one stream, or events).  Arguments that
+ * the host can see are checked before anything is launched (BRISK_HIP_EINVAL);
+ * what lies in device memory is bounds-checked by the kernels, which leave out
+ * what it names beyond the tensors, the tables or the cache. */
+
+/* A tensor [rows][heads][head_dim]: F32, F16 or BF16, a head's values
+ * contiguous, strides in values; `data` is aligned to its type.  Any strides are read; rows and heads that
+ * are written do not overlap. */
+typedef struct {
+    void* data;
+    int type;
+    size_t row_stride, head_stride;
+} brisk_hip_heads;
+
+/* Rotations: (cos, sin) pairs [positions][dims / 2] in f32, the layout of the
+ * sessions' own tables (src/model.cpp:880-894); a scaling for long contexts,
+ * frequency factors or a magnitude are in its values.  The first `dims` values
+ * of a head turn, in pairs (i, i + dims / 2) for neox 1, (2 i, 2 i + 1) for
+ * neox 2, as brisk_hip_config::rope_neox. */
+typedef struct {
+    const float* table;
+    uint32_t positions, dims;
+    int32_t neox;
+} brisk_hip_rope;
+
+/* A cache of `pages` pages of page_tokens positions (a power of two, 16 to
+ * 1024) of every key/value head; head_dim 64, 96, 128, 256 or 512.  `type` is
+ * BRISK_HIP_F16 (rounded to nearest; past its range infinite) or
+ * BRISK_HIP_Q4_0: blocks of 32 values of a head, held as that format holds
+ * them: a scale d, the first value of largest magnitude over -8 rounded to
+ * fp16, and codes n = floor(x / d + 8.5) within 0..15; a code stands for
+ * (n - 8) d.  A 4-bit block with a value that is not finite, or that needs
+ * a scale over 8188 (values past fp16's range, 65504), reads as NaN.  The values are arranged for the
+ * attention's loads: brisk_hip_kv_append writes them, brisk_hip_kv_read gives
+ * them back.  `data`: brisk_hip_kv_bytes() bytes, 16-byte aligned; it needs no
+ * initialisation. */
+typedef struct {
+    void* data;
+    int type;
+    uint32_t kv_heads, head_dim, page_tokens, pages;
+} brisk_hip_kv;
+
+/* Sequences and their rows.  Rows row_start[s] .. row_start[s + 1] - 1 of a
+ * call's tensors (rows in all) belong to sequence s and are its last positions:
+ * the last of them is position lengths[s] - 1.  Position p is held in page
+ * page_table[s * page_stride + p / page_tokens].  Rows before position 0 (more
+ * rows than the length), rows of no sequence and rows past `rows` are left out; a position whose
+ * entry is not a page, or that the table does not reach, holds nothing.
+ * max_rows and max_length are the host's bounds of a sequence's rows and length
+ * (0: not known): they size the launches, and results do not depend on their
+ * being right. */
+typedef struct {
+    const int32_t* row_start;  /* [seqs + 1] */
+    const int32_t* lengths;    /* [seqs] */
+    const int32_t* page_table; /* [seqs][page_stride] */
+    uint32_t seqs, rows, page_stride, max_rows, max_length;
+} brisk_hip_batch;
+
+/* Bytes of a cache (its `data` is not looked at); 0 for a shape or type that is not taken. */
+size_t brisk_hip_kv_bytes(const brisk_hip_kv* kv);
+
+/* Queries and keys, each head RMS-normalised (q_norm / k_norm: head_dim
+ * weights, NULL: not; src/model.cpp:87-97, :1020-1046) and rotated by its row's
+ * position (rope NULL: not), in one pass and in f32.  k and k_out may be NULL.
+ * Rows whose position is outside the table are left as they were, so -1 marks
+ * padding; positions may be NULL without rope.  An output may be its own input
+ * (the same data, type and strides).  head_dim: a multiple of 8, at most 512. */
+int brisk_hip_qk_norm_rope(const brisk_hip_heads* q, const brisk_hip_heads* k, size_t n, uint32_t heads, uint32_t kv_heads,
+                           uint32_t head_dim, const float* q_norm, const float* k_norm, float eps, const brisk_hip_rope* rope,
+                           const int32_t* positions, const brisk_hip_heads* q_out, const brisk_hip_heads* k_out,
+                           void* stream);
+
+/* Appends the batch's rows of keys (normed and rotated on the way, as above, by
+ * their positions) and values to their pages.  A row whose position is outside
+ * the rotation's table is not stored.  Rows of different sequences go to
+ * different pages: of two rows that name one place, parts of either may be kept. */
+int brisk_hip_kv_append(const brisk_hip_kv* kv, const brisk_hip_batch* batch, const brisk_hip_heads* k, const brisk_hip_heads* v,
+                        const float* k_norm, float eps, const brisk_hip_rope* rope, void* stream);
+
+/* Reads the cached keys and values at the positions of the batch's rows (a
+ * whole sequence's, when its rows are its length); k or v may be NULL.  Rows
+ * that the cache does not hold are left as they were.  With the strides of a
+ * session's cache (brisk_hip_session_kv_cache) it restores one from pages, and
+ * brisk_hip_kv_append takes one in. */
+int brisk_hip_kv_read(const brisk_hip_kv* kv, const brisk_hip_batch* batch, const brisk_hip_heads* k, const brisk_hip_heads* v,
+                      void* stream);
+
+/* Workspace of brisk_hip_paged_attention for this cache, batch (its device arrays are not
+ * looked at) and head count; may be 0. */
+size_t brisk_hip_paged_attention_bytes(const brisk_hip_kv* kv, const brisk_hip_batch* batch, uint32_t heads);
+
+/* Causal attention of the batch's rows over their sequences' cached positions
+ * (src/model.cpp:1050-1093): row at position p sees positions max(0, p - window
+ * + 1) .. p (window 0: from 0), query head h reads key/value head
+ * h / (heads / kv_heads), and out = sum softmax(scale q k) v.  What a row does not see has no part
+ * in it, infinities and NaN included; a row that sees nothing, or only scores of
+ * minus infinity, gives zeros.  q, out: [rows][heads][head_dim]; with 16-bit
+ * queries and outputs, queries and probabilities are multiplied in 16 bits and
+ * summed in 32; with F32 queries or outputs the products are those of 32 bits.
+ * `workspace`: brisk_hip_paged_attention_bytes() bytes at least, 16-byte
+ * aligned, used by this call alone while it runs (NULL where 0 are needed). */
+int brisk_hip_paged_attention(const brisk_hip_kv* kv, const brisk_hip_batch* batch, const brisk_hip_heads* q, uint32_t heads,
+                              float scale, uint32_t window, const brisk_hip_heads* out, void* workspace, size_t workspace_bytes,
+                              void* stream);
 
 /* ---------------------------------------------------------------- session level */
 
