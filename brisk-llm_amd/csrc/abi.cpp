@@ -442,7 +442,10 @@ int brisk_hip_paged_attention(const brisk_hip_kv* kv, const brisk_hip_batch* bat
         bh::PagedAttnArgs a{};
         a.kv = paged_kv(kv, true);
         a.b = paged_batch(batch, true);
-        a.group = head_group(heads, a.kv);
+        a.group = bh::divisor(head_group(heads, a.kv));
+        a.per_row = bh::divisor(heads);
+        a.kv_heads = bh::divisor(a.kv.kv_heads);
+        if (static_cast<uint64_t>(a.b.rows) * heads > 0x7FFFFFFFu) bad("too many rows and heads");
         if (!std::isfinite(scale)) bad("the score scale must be finite");
         if (a.b.rows == 0 || a.b.seqs == 0) return;
         a.heads = heads;

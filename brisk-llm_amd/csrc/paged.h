@@ -74,38 +74,37 @@ BH_BOTH uint32_t tile_values_at(bool q4, uint32_t nb) { return q4 ? 256 * nb : 1
 BH_BOTH uint32_t tile_key_scales_at(uint32_t nb) { return 512 * nb; }
 BH_BOTH uint32_t tile_value_scales_at(uint32_t nb) { return 544 * nb; }
 
-// A sequence's rows in the batch's tensors and the position of row r, as (row_start + r) - first: a
-// row table that is out of order or past the tensors gives no rows outside them.
+// A sequence's rows in the batch's tensors and their positions.  A row table that is out of order or
+// past the tensors gives no rows outside them; positions stay below kMaxLength.
+constexpr int32_t kMaxLength = 0x7FFFFC00;
 struct SeqRows {
-    int64_t begin, end;  // rows of the tensors
-    int64_t first;       // position of row `begin`; negative positions hold nothing
-    int64_t length;
+    int32_t begin, end;  // rows of the tensors
+    int32_t first;       // position of row `begin`; negative positions hold nothing
 };
 BH_BOTH SeqRows seq_rows(const PagedBatch& b, uint32_t s) {
-    const int64_t lo = b.row_start[s], hi = b.row_start[s + 1];
+    const int32_t lo = b.row_start[s], hi = b.row_start[s + 1], n = b.lengths[s];
+    const int32_t length = n < 0 ? 0 : n > kMaxLength ? kMaxLength : n, rows = static_cast<int32_t>(b.rows);
     SeqRows q;
-    q.length = b.lengths[s] < 0 ? 0 : b.lengths[s];
     q.begin = lo < 0 ? 0 : lo;
-    q.end = hi > static_cast<int64_t>(b.rows) ? static_cast<int64_t>(b.rows) : hi;
+    q.end = hi > rows ? rows : hi;
     if (q.end < q.begin) q.end = q.begin;
-    q.first = q.length - (hi - q.begin);
+    q.first = length - (hi < q.begin ? 0 : hi - q.begin);
     return q;
 }
 
 // The page of a position, or -1: a position outside the table's row, or an entry that names no page.
-BH_BOTH int64_t page_of(const PagedKv& kv, const PagedBatch& b, uint32_t s, int64_t pos) {
+BH_BOTH int32_t page_of(const PagedKv& kv, const PagedBatch& b, uint32_t s, int32_t pos) {
     if (pos < 0) return -1;
-    const uint64_t e = static_cast<uint64_t>(pos) >> kv.page_shift;
+    const uint32_t e = static_cast<uint32_t>(pos) >> kv.page_shift;
     if (e >= b.page_stride) return -1;
     const int32_t p = b.page_table[static_cast<size_t>(s) * b.page_stride + e];
     return p < 0 || static_cast<uint32_t>(p) >= kv.pages ? -1 : p;
 }
 
 // Byte offset of the tile of position `pos` of head h in page `page`.
-BH_BOTH size_t tile_at(const PagedKv& kv, int64_t page, uint32_t h, int64_t pos) {
-    const uint32_t per = kv.page_tokens / kTileTokens;
+BH_BOTH size_t tile_at(const PagedKv& kv, int32_t page, uint32_t h, int32_t pos) {
     const uint32_t t = (static_cast<uint32_t>(pos) & (kv.page_tokens - 1)) / kTileTokens;
-    return ((static_cast<size_t>(page) * kv.kv_heads + h) * per + t) * tile_bytes(kv.q4 != 0, kv.head_dim / 32);
+    return ((static_cast<size_t>(static_cast<uint32_t>(page)) * kv.kv_heads + h) * (kv.page_tokens / kTileTokens) + t) * tile_bytes(kv.q4 != 0, kv.head_dim / 32);
 }
 
 // Offsets in a tile.  `d` is a multiple of 8 for the keys (eight values: 16 bytes, or a word) and of
@@ -122,6 +121,18 @@ BH_BOTH uint32_t value_offset(bool q4, uint32_t nb, uint32_t token, uint32_t d) 
 BH_BOTH uint32_t scale_offset(uint32_t nb, bool value, uint32_t token, uint32_t b) {
     return (value ? tile_value_scales_at(nb) : tile_key_scales_at(nb)) + ((token / 4 * nb + b) * 4 + token % 4) * 2;
 }
+
+// Division of numbers below 2^31 by a divisor known when a kernel is launched: n * m >> s with m =
+// ceil(2^s / d) and s = 31 + ceil(log2 d), which is exact there.
+struct Divisor {
+    uint32_t d, m, s;
+};
+BH_BOTH Divisor divisor(uint32_t d) {
+    uint32_t s = 31;
+    while ((uint64_t{1} << (s - 31)) < d) ++s;
+    return {d, static_cast<uint32_t>(((uint64_t{1} << s) + d - 1) / d), s};
+}
+BH_BOTH uint32_t over(uint32_t n, const Divisor& d) { return static_cast<uint32_t>(static_cast<uint64_t>(n) * d.m >> d.s); }
 
 #ifdef __HIPCC__
 
@@ -157,7 +168,8 @@ struct PagedAttnArgs {
     PagedKv kv;
     PagedBatch b;
     HeadRows q, out;
-    uint32_t heads, group;
+    uint32_t heads;
+    Divisor group, per_row, kv_heads;  // query heads of a key/value head, query heads, key/value heads
     float scale;
     uint32_t window;  // 0: none
     uint32_t splits;

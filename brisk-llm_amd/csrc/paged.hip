@@ -174,19 +174,19 @@ __global__ __launch_bounds__(kThreads) void k_kv_append(AppendArgs a, int lanes,
     const int64_t per = kThreads / lanes, heads = a.kv.kv_heads;
     for (uint32_t s = blockIdx.y; s < a.b.seqs; s += gridDim.y) {
         const SeqRows sr = seq_rows(a.b, s);
-        const int64_t total = (sr.end - sr.begin) * heads * 2;
+        const int64_t total = static_cast<int64_t>(sr.end - sr.begin) * heads * 2;
         for (int64_t base = blockIdx.x * per; base < total; base += static_cast<int64_t>(gridDim.x) * per) {
             const int64_t u = base + threadIdx.x / lanes;
             const bool in = u < total;
             const int64_t row = sr.begin + (in ? u / (2 * heads) : 0);
             const uint32_t h = in ? static_cast<uint32_t>(u % heads) : 0;
             const bool value = in && u % (2 * heads) >= heads;
-            const int64_t pos = sr.first + (row - sr.begin);
-            const int64_t page = page_of(a.kv, a.b, s, pos);
+            const int32_t pos = sr.first + static_cast<int32_t>(row - sr.begin);
+            const int32_t page = page_of(a.kv, a.b, s, pos);
             bool keep = !in || page < 0;
             const float* cs = nullptr;
             if (a.rope.table != nullptr) {
-                if (pos < 0 || pos >= static_cast<int64_t>(a.rope.positions)) keep = true;
+                if (pos < 0 || static_cast<uint32_t>(pos) >= a.rope.positions) keep = true;
                 else cs = a.rope.table + static_cast<size_t>(pos) * a.rope.dims;
             }
             const HeadRows& x = value ? a.v : a.k;
@@ -230,13 +230,13 @@ __global__ __launch_bounds__(kThreads) void k_kv_read(ReadArgs a, int lanes, int
     const int64_t per = kThreads / lanes, heads = a.kv.kv_heads;
     for (uint32_t s = blockIdx.y; s < a.b.seqs; s += gridDim.y) {
         const SeqRows sr = seq_rows(a.b, s);
-        const int64_t total = (sr.end - sr.begin) * heads * 2;
+        const int64_t total = static_cast<int64_t>(sr.end - sr.begin) * heads * 2;
         for (int64_t u = blockIdx.x * per + threadIdx.x / lanes; u < total; u += static_cast<int64_t>(gridDim.x) * per) {
             const int64_t row = sr.begin + u / (2 * heads);
             const uint32_t h = static_cast<uint32_t>(u % heads);
             const bool value = u % (2 * heads) >= heads;
             const HeadRows& y = value ? a.v : a.k;
-            const int64_t pos = sr.first + (row - sr.begin), page = page_of(a.kv, a.b, s, pos);
+            const int32_t pos = sr.first + static_cast<int32_t>(row - sr.begin), page = page_of(a.kv, a.b, s, pos);
             if (y.data == nullptr || page < 0) continue;
             const uint8_t* tile = a.kv.data + tile_at(a.kv, page, h, pos);
             const uint32_t token = static_cast<uint32_t>(pos) % kTileTokens;

@@ -53,127 +53,236 @@ __device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {
     for (int k = 0; k < N; ++k) w[k] = x.w[k];
 }
 
-// EXACT: queries and probabilities as sums of two halves, and 4-bit values as sums of two: 32-bit results.
+// What a wave holds of two tiles: keys, values and, of 4-bit tiles, their scales.
+template <int NB, bool Q4>
+struct TilePair {
+    static constexpr int GS = NB < 4 ? NB : 4, NG = NB / GS;
+    uint32_t k[2][NG][Q4 ? GS : 4 * GS], v[2][NG][Q4 ? 1 : 4][GS];
+    uint32_t ks[2][NG][Q4 ? 2 * GS : 1], vs[2][NG][Q4 ? 2 * GS : 1];
+
+    __device__ inline void load_keys(const uint8_t* tile, int x, int lane) {
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            if constexpr (Q4) {
+                load_words<GS>(tile + (n * 64 + lane) * GS * 4, k[x][n]);
+                load_words<2 * GS>(tile + tile_key_scales_at(NB) + (lane / 16 * NB + n * GS) * 8, ks[x][n]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < GS; ++j) {
+                    const word4v w = *reinterpret_cast<const word4v*>(tile + ((n * GS + j) * 64 + lane) * 16);
+                    for (int e = 0; e < 4; ++e) k[x][n][4 * j + e] = w[e];
+                }
+            }
+        }
+    }
+    __device__ inline void load_values(const uint8_t* tile, int x, int n, int lane) {
+        const uint8_t* at = tile + tile_values_at(Q4, NB);
+        if constexpr (Q4) {
+            load_words<GS>(at + (n * 64 + lane) * GS * 4, v[x][n][0]);
+            load_words<2 * GS>(tile + tile_value_scales_at(NB) + (lane / 16 * NB + n * GS) * 8, vs[x][n]);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) load_words<GS>(at + ((r * NG + n) * 64 + lane) * GS * 4, v[x][n][r]);
+        }
+    }
+    // Leaves out the values of positions whose bit 4 x + r of `seen` is not set, whatever lies there.
+    __device__ inline void keep_seen(int n, uint32_t seen) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            if constexpr (Q4) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t b = seen >> (4 * x + 2 * j), mask = (b & 1 ? 0xFFFF : 0) | (b & 2 ? 0xFFFF0000 : 0);
+                    for (int k = 0; k < GS; ++k) vs[x][n][2 * k + j] &= mask;
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t mask = seen >> (4 * x + r) & 1 ? 0xFFFFFFFF : 0;
+                    for (int k = 0; k < GS; ++k) v[x][n][r][k] &= mask;
+                }
+            }
+        }
+    }
+    // Infinities and NaN among a group of blocks' values, and the values without them.
+    __device__ inline bool any_ill(int n) const {
+        uint32_t found = 0;
+        for (int x = 0; x < 2; ++x) {
+            if constexpr (Q4) {
+                for (int j = 0; j < 2 * GS; ++j) found |= ill<true>(vs[x][n][j]);
+            } else {
+                for (int r = 0; r < 4; ++r)
+                    for (int j = 0; j < GS; ++j) found |= ill<false>(v[x][n][r][j]);
+            }
+        }
+        return __any((found & kIll) != 0);
+    }
+    __device__ inline void drop_ill(int n) {
+        for (int x = 0; x < 2; ++x) {
+            if constexpr (Q4) {
+                for (int j = 0; j < 2 * GS; ++j) vs[x][n][j] = without_ill<true>(vs[x][n][j]);
+            } else {
+                for (int r = 0; r < 4; ++r)
+                    for (int j = 0; j < GS; ++j) v[x][n][r][j] = without_ill<false>(v[x][n][r][j]);
+            }
+        }
+    }
+};
+
+// A workgroup takes up to 16 columns, the (row, head) pairs of one key/value head, and one part of the
+// positions they see; its waves take pairs of tiles in turn.  EXACT: queries and probabilities as sums
+// of two halves, and 4-bit values as sums of two: 32-bit results.
 template <int NB, bool Q4, bool EXACT>
-__global__ __launch_bounds__(64 * kWaves) void k_paged_attn(PagedAttnArgs a) {
-    constexpr int GS = NB < 4 ? NB : 4, NG = NB / GS, HD = 32 * NB;
-    __shared__ float merge[kWaves][kColumns][kMergeRow];
-    __shared__ float stats[kWaves][kColumns][2];
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(NB <= 2 ? 4 : NB <= 4 ? 3 : NB <= 8 ? 2 : 1))) void k_paged_attn(PagedAttnArgs a) {
+    constexpr int GS = NB < 4 ? NB : 4, NG = NB / GS, HD = 32 * NB, QROW = HD + 8;
+    constexpr bool kEarly = NB <= 8;  // all of a pair's loads ahead of its products (the widest heads have no registers for it)
+    constexpr bool kHeldQ = NB * (EXACT ? 2 : 1) <= 8;  // queries in registers, otherwise read from LDS for each product
+    __shared__ union {
+        _Float16 q[EXACT ? 2 : 1][kColumns][QROW];
+        float merge[kWaves][kColumns][kMergeRow];
+    } lds;
+    __shared__ float qfactor[kColumns], stats[kWaves][kColumns][2];
     const int lane = static_cast<int>(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int i = lane % 16, g = lane / 16;
-    const uint32_t h = blockIdx.y % a.kv.kv_heads, first_tile = blockIdx.y / a.kv.kv_heads, tiles = gridDim.y / a.kv.kv_heads;
-    const int64_t window = a.window;
+    const uint32_t first_tile = over(blockIdx.y, a.kv_heads), h = blockIdx.y - first_tile * a.kv.kv_heads;
+    const int32_t window = a.window > static_cast<uint32_t>(kMaxLength) ? 0 : static_cast<int32_t>(a.window);
 
     for (uint32_t s = blockIdx.z; s < a.b.seqs; s += gridDim.z) {
         const SeqRows sr = seq_rows(a.b, s);
-        const int64_t cols = (sr.end - sr.begin) * a.group;
-        for (int64_t ct = first_tile; ct * kColumns < cols; ct += tiles) {
-            const int64_t c = ct * kColumns + i, last = std::min<int64_t>(ct * kColumns + kColumns, cols) - 1;
-            const bool mine = c < cols;
-            const int64_t row = sr.begin + (mine ? c / a.group : 0);
-            const int64_t head = static_cast<int64_t>(h) * a.group + (mine ? c % a.group : 0);
-            const int64_t pos_lo = sr.first + ct * kColumns / a.group, pos_hi = sr.first + last / a.group;
-            const int64_t pos = mine ? sr.first + (row - sr.begin) : pos_lo;
-            const int64_t t_lo = window != 0 && pos_lo - window + 1 > 0 ? pos_lo - window + 1 : 0;
-            const int64_t t_hi = std::min<int64_t>(pos_hi + 1, static_cast<int64_t>(a.b.page_stride) << a.kv.page_shift);
-            const int64_t step_lo = t_lo / kStep, steps = t_hi > t_lo ? (t_hi + kStep - 1) / kStep - step_lo : 0;
-            const int64_t per = (steps + a.splits - 1) / a.splits;
-            const int64_t step_end = step_lo + std::min<int64_t>(steps, per * (blockIdx.x + 1));
+        const uint32_t cols = (sr.end - sr.begin) * a.group.d;
+        for (uint32_t c0 = first_tile * kColumns; c0 < cols; c0 += over(gridDim.y, a.kv_heads) * kColumns) {
+            const uint32_t c_last = std::min<uint32_t>(c0 + kColumns, cols) - 1;
+            const int32_t pos_lo = sr.first + static_cast<int32_t>(over(c0, a.group)), pos_hi = sr.first + static_cast<int32_t>(over(c_last, a.group));
+            const int32_t t_lo = window != 0 && pos_lo - window + 1 > 0 ? pos_lo - window + 1 : 0;
+            const int32_t t_hi = static_cast<int32_t>(std::min<int64_t>(static_cast<int64_t>(pos_hi) + 1, static_cast<int64_t>(a.b.page_stride) << a.kv.page_shift));
+            const int32_t step_lo = t_lo / kStep, steps = t_hi > t_lo ? (t_hi + kStep - 1) / kStep - step_lo : 0;
+            const int32_t per = (steps + static_cast<int32_t>(a.splits) - 1) / static_cast<int32_t>(a.splits);
+            const int32_t step_end = step_lo + static_cast<int32_t>(std::min<int64_t>(steps, static_cast<int64_t>(per) * (blockIdx.x + 1)));
+            int32_t step = step_lo + per * static_cast<int32_t>(blockIdx.x) + wave;
+            int32_t page[2] = {-1, -1};
+            if (step < step_end) {
+                page[0] = page_of(a.kv, a.b, s, step * kStep);
+                page[1] = page_of(a.kv, a.b, s, step * kStep + 16);
+            }
 
-            // the column's query, scaled by a power of two where its type has more range than a half
-            half8v qh[NB], ql[EXACT ? NB : 1];
-            float qscale = a.scale * 1.44269504088896f;
+            // the columns' queries, as halves in LDS: 16 threads a column, scaled by a power of two where
+            // the type has more range than a half
             {
-                const char* qp = row_ptr(a.q, row, head);
-                const bool vec = (reinterpret_cast<uintptr_t>(qp) & 15) == 0;
-                float top = 0;
-                float x[NB][8];
+                const uint32_t qc = threadIdx.x / 16, sub = threadIdx.x % 16, c = c0 + qc, row = over(c, a.group);
+                constexpr int K = (HD + 127) / 128;
+                float x[K][8], top = 0;
+                const char* qp = row_ptr(a.q, sr.begin + row, h * a.group.d + (c - row * a.group.d));
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    load8(qp, a.q.type, vec, 32 * b + 8 * g, x[b]);
+                for (int k = 0; k < K; ++k) {
+                    for (int j = 0; j < 8; ++j) x[k][j] = 0;
+                    const int d = (k * 16 + sub) * 8;
+                    if (c < cols && d < HD) load8(qp, a.q.type, (reinterpret_cast<uintptr_t>(qp) & 15) == 0, d, x[k]);
+                    for (int j = 0; j < 8; ++j) top = __builtin_fmaxf(top, __builtin_fabsf(x[k][j]));
+                }
+                for (int m = 1; m < 16; m *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, m));
+                const int e = a.q.type != kTypeF16 && top > 0 && top <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(top) : 9;
+                if (sub == 0) qfactor[qc] = __builtin_ldexpf(a.scale * 1.44269504088896f, e - 9);
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const int d = (k * 16 + sub) * 8;
+                    half8v hi, lo;
                     for (int j = 0; j < 8; ++j) {
-                        if (!mine) x[b][j] = 0;
-                        top = __builtin_fmaxf(top, __builtin_fabsf(x[b][j]));
+                        const float y = __builtin_ldexpf(x[k][j], 9 - e);
+                        hi[j] = static_cast<_Float16>(y);
+                        lo[j] = static_cast<_Float16>(y - static_cast<float>(hi[j]));
                     }
-                }
-                int e = 9;
-                if (a.q.type != kTypeF16) {
-                    top = __builtin_fmaxf(top, __shfl_xor(top, 16));
-                    top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-                    if (top > 0 && top <= 3.402823466e38f) e = __builtin_amdgcn_frexp_expf(top);
-                }
-                qscale = __builtin_ldexpf(qscale, e - 9);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    for (int j = 0; j < 8; ++j) {
-                        const float y = __builtin_ldexpf(x[b][j], 9 - e);
-                        qh[b][j] = static_cast<_Float16>(y);
-                        if constexpr (EXACT) ql[b][j] = static_cast<_Float16>(y - static_cast<float>(qh[b][j]));
+                    if (d < HD) {
+                        *reinterpret_cast<half8v*>(&lds.q[0][qc][d]) = hi;
+                        if constexpr (EXACT) *reinterpret_cast<half8v*>(&lds.q[1][qc][d]) = lo;
                     }
                 }
             }
+            __syncthreads();
+            half8v held[EXACT ? 2 : 1][kHeldQ ? NB : 1];
+            if constexpr (kHeldQ) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    for (int e = 0; e < (EXACT ? 2 : 1); ++e) held[e][b] = *reinterpret_cast<const half8v*>(&lds.q[e][i][32 * b + 8 * g]);
+                }
+            }
+            const auto query = [&](int part, int b) -> half8v {
+                if constexpr (kHeldQ) return held[part][b];
+                else return *reinterpret_cast<const half8v*>(&lds.q[part][i][32 * b + 8 * g]);
+            };
+            const float qscale = qfactor[i];
+            const int32_t pos = c0 + i < cols ? sr.first + static_cast<int32_t>(over(c0 + i, a.group)) : pos_lo;
 
             float m = -__builtin_inff(), l = 0;
             float4v acc[NB][2];
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[b][0] = acc[b][1] = float4v{0, 0, 0, 0};
 
-            for (int64_t step = step_lo + per * blockIdx.x + wave; step < step_end; step += kWaves) {
-                const int64_t t0 = step * kStep;
+            for (; step < step_end; step += kWaves) {
+                const int32_t t0 = step * kStep;
                 const uint8_t* tile[2];
                 bool there[2];
+                TilePair<NB, Q4> kv;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    there[x] = page[x] >= 0;
+                    tile[x] = a.kv.data + tile_at(a.kv, there[x] ? page[x] : 0, h, t0 + 16 * x);
+                    if constexpr (kEarly) kv.load_keys(tile[x], x, lane);
+                }
+                if constexpr (kEarly) {
+#pragma unroll
+                    for (int n = 0; n < NG; ++n) {
+                        kv.load_values(tile[0], 0, n, lane);
+                        kv.load_values(tile[1], 1, n, lane);
+                    }
+                }
+                if (step + kWaves < step_end) {
+                    page[0] = page_of(a.kv, a.b, s, t0 + kWaves * kStep);
+                    page[1] = page_of(a.kv, a.b, s, t0 + kWaves * kStep + 16);
+                }
                 float4v sc[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const int64_t page = page_of(a.kv, a.b, s, t0 + 16 * x);
-                    there[x] = page >= 0;
-                    tile[x] = a.kv.data + tile_at(a.kv, page < 0 ? 0 : page, h, t0 + 16 * x);
-                    float4v sum{0, 0, 0, 0};
-                    if constexpr (Q4) {
+                    sc[x] = float4v{0, 0, 0, 0};
+                    if constexpr (!kEarly) kv.load_keys(tile[x], x, lane);
 #pragma unroll
-                        for (int n = 0; n < NG; ++n) {
-                            uint32_t w[GS];
-                            load_words<GS>(tile[x] + (n * 64 + lane) * GS * 4, w);
-#pragma unroll
-                            for (int k = 0; k < GS; ++k) {
-                                const int b = n * GS + k;
-                                const half8v kx = operand(bits(codes(w[k], false)), bits(codes(w[k], true)), bits(codes(w[k] >> 8, false)),
-                                                          bits(codes(w[k] >> 8, true)));
-                                float4v d{0, 0, 0, 0};
-                                if constexpr (EXACT) d = mfma(kx, ql[b], d);
-                                d = mfma(kx, qh[b], d);
-                                const word2v ks = *reinterpret_cast<const word2v*>(tile[x] + tile_key_scales_at(NB) + (g * NB + b) * 8);
-                                sum[0] = __builtin_fmaf(d[0], from_half(ks[0] & 0xFFFF), sum[0]);
-                                sum[1] = __builtin_fmaf(d[1], from_half(ks[0] >> 16), sum[1]);
-                                sum[2] = __builtin_fmaf(d[2], from_half(ks[1] & 0xFFFF), sum[2]);
-                                sum[3] = __builtin_fmaf(d[3], from_half(ks[1] >> 16), sum[3]);
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            const half8v kx = __builtin_bit_cast(half8v, *reinterpret_cast<const word4v*>(tile[x] + (b * 64 + lane) * 16));
-                            if constexpr (EXACT) sum = mfma(kx, ql[b], sum);
-                            sum = mfma(kx, qh[b], sum);
+                    for (int b = 0; b < NB; ++b) {
+                        const int n = b / GS, k = b % GS;
+                        if constexpr (Q4) {
+                            const uint32_t w = kv.k[x][n][k], w8 = w >> 8;
+                            const half8v kx = operand(bits(codes(w, false)), bits(codes(w, true)), bits(codes(w8, false)), bits(codes(w8, true)));
+                            float4v d{0, 0, 0, 0};
+                            if constexpr (EXACT) d = mfma(kx, query(1, b), d);
+                            d = mfma(kx, query(0, b), d);
+                            const half2v s01 = halves(kv.ks[x][n][2 * k]), s23 = halves(kv.ks[x][n][2 * k + 1]);
+                            sc[x][0] = __builtin_fmaf(d[0], static_cast<float>(s01[0]), sc[x][0]);
+                            sc[x][1] = __builtin_fmaf(d[1], static_cast<float>(s01[1]), sc[x][1]);
+                            sc[x][2] = __builtin_fmaf(d[2], static_cast<float>(s23[0]), sc[x][2]);
+                            sc[x][3] = __builtin_fmaf(d[3], static_cast<float>(s23[1]), sc[x][3]);
+                        } else {
+                            const half8v kx = operand(kv.k[x][n][4 * k], kv.k[x][n][4 * k + 1], kv.k[x][n][4 * k + 2], kv.k[x][n][4 * k + 3]);
+                            if constexpr (EXACT) sc[x] = mfma(kx, query(1, b), sc[x]);
+                            sc[x] = mfma(kx, query(0, b), sc[x]);
                         }
                     }
-                    sc[x] = sum;
                 }
                 // positions t0 .. t0 + 31 that every column sees need no masks
                 const bool full = there[0] && there[1] && t0 + kStep - 1 <= pos_lo && (window == 0 || t0 > pos_hi - window);
                 float p[8];
-                uint32_t seen = 0xFF;
+                uint32_t seen = 0xFF, anyones = 0xFF;  // of the lane's positions, by its column and by any
+                if (!full) {
+                    seen = anyones = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int32_t t = t0 + 16 * (j / 4) + 4 * g + j % 4;
+                        if (there[j / 4] && t >= t_lo && t <= pos_hi) anyones |= 1u << j;
+                        if (there[j / 4] && t <= pos && (window == 0 || t > pos - window)) seen |= 1u << j;
+                        else sc[j / 4][j % 4] = qscale < 0 ? __builtin_inff() : -__builtin_inff();
+                    }
+                }
                 float top = -__builtin_inff();
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     p[j] = sc[j / 4][j % 4] * qscale;
-                    if (!full) {
-                        const int64_t t = t0 + 16 * (j / 4) + 4 * g + j % 4;
-                        if (!(there[j / 4] && t <= pos && (window == 0 || t > pos - window))) {
-                            p[j] = -__builtin_inff();
-                            seen &= ~(1u << j);
-                        }
-                    }
                     top = __builtin_fmaxf(top, p[j]);
                 }
                 if (__any(top > m + kLazy)) {
@@ -198,46 +307,21 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn(PagedAttnArgs a) {
                     ph[j] = static_cast<_Float16>(p[j]);
                     if constexpr (EXACT) pl[j] = static_cast<_Float16>(p[j] - static_cast<float>(ph[j]));
                 }
-                // a value that is not finite, at a position that some column does not see: the product
-                // is taken without it, and the columns that see it get it afterwards (4-bit: its whole block is NaN)
                 bool poison = false;
 #pragma unroll
                 for (int n = 0; n < NG; ++n) {
-                    uint32_t v[2][Q4 ? 1 : 4][GS], vs[2][Q4 ? 2 * GS : 1];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint8_t* at = tile[x] + tile_values_at(Q4, NB);
-                        if constexpr (Q4) {
-                            load_words<GS>(at + (n * 64 + lane) * GS * 4, v[x][0]);
-                            load_words<2 * GS>(tile[x] + tile_value_scales_at(NB) + (g * NB + n * GS) * 8, vs[x]);
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) load_words<GS>(at + ((r * NG + n) * 64 + lane) * GS * 4, v[x][r]);
-                        }
+                    if constexpr (!kEarly) {
+                        kv.load_values(tile[0], 0, n, lane);
+                        kv.load_values(tile[1], 1, n, lane);
                     }
-                    // (with 32-bit results everywhere: an infinity times a probability's second part is of any sign)
+                    if (!full) kv.keep_seen(n, anyones);
+                    // a value that is not finite, at a position that some column does not see: the product is
+                    // taken without it, and the columns that see it get it afterwards (4-bit: its whole block is
+                    // NaN).  With 32-bit results everywhere: an infinity times a probability's second part is of any sign
                     if (!full || (EXACT && !Q4)) {
-                        uint32_t found = 0;
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            if constexpr (Q4) {
-                                for (int k = 0; k < 2 * GS; ++k) found |= ill<true>(vs[x][k]);
-                            } else {
-                                for (int r = 0; r < 4; ++r)
-                                    for (int k = 0; k < GS; ++k) found |= ill<false>(v[x][r][k]);
-                            }
-                        }
-                        if (__any((found & kIll) != 0)) {
+                        if (kv.any_ill(n)) {
+                            kv.drop_ill(n);
                             poison = true;
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                if constexpr (Q4) {
-                                    for (int k = 0; k < 2 * GS; ++k) vs[x][k] = without_ill<true>(vs[x][k]);
-                                } else {
-                                    for (int r = 0; r < 4; ++r)
-                                        for (int k = 0; k < GS; ++k) v[x][r][k] = without_ill<false>(v[x][r][k]);
-                                }
-                            }
                         }
                     }
 #pragma unroll
@@ -249,8 +333,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn(PagedAttnArgs a) {
 #pragma unroll
                             for (int x = 0; x < 2; ++x) {
                                 if constexpr (Q4) {
-                                    const half2v c01 = codes(v[x][0][k], c2), c23 = codes(v[x][0][k] >> 8, c2);
-                                    const half2v d01 = halves(vs[x][2 * k]), d23 = halves(vs[x][2 * k + 1]);
+                                    const uint32_t w = kv.v[x][n][0][k];
+                                    const half2v c01 = codes(w, c2), c23 = codes(w >> 8, c2);
+                                    const half2v d01 = halves(kv.vs[x][n][2 * k]), d23 = halves(kv.vs[x][n][2 * k + 1]);
                                     const half2v v01 = c01 * d01, v23 = c23 * d23;
                                     hi[2 * x] = bits(v01);
                                     hi[2 * x + 1] = bits(v23);
@@ -261,8 +346,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn(PagedAttnArgs a) {
                                     }
                                 } else {
                                     const uint32_t sel = c2 ? 0x07060302 : 0x05040100;
-                                    hi[2 * x] = __builtin_amdgcn_perm(v[x][1][k], v[x][0][k], sel);
-                                    hi[2 * x + 1] = __builtin_amdgcn_perm(v[x][3][k], v[x][2][k], sel);
+                                    hi[2 * x] = __builtin_amdgcn_perm(kv.v[x][n][1][k], kv.v[x][n][0][k], sel);
+                                    hi[2 * x + 1] = __builtin_amdgcn_perm(kv.v[x][n][3][k], kv.v[x][n][2][k], sel);
                                 }
                             }
                             const half8v vh = operand(hi[0], hi[1], hi[2], hi[3]);
@@ -274,16 +359,20 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn(PagedAttnArgs a) {
                         }
                     }
                 }
-                if (poison) {
+                if (__builtin_expect(poison, 0)) {
+#pragma unroll 1
                     for (int j = 0; j < 8; ++j) {
+#pragma unroll 1
                         for (int gg = 0; gg < 4; ++gg) {
-                            const float pt = __shfl(p[j], i + 16 * gg);
+                            float pt = 0;
+#pragma unroll
+                            for (int y = 0; y < 8; ++y) pt = y == j ? p[y] : pt;
+                            pt = __shfl(pt, i + 16 * gg);
                             const bool sees = __shfl(seen, i + 16 * gg) >> j & 1;
-                            const uint32_t token = 4 * gg + j % 4;
 #pragma unroll
                             for (int b = 0; b < NB; ++b) {
                                 float x[8];
-                                read8(tile[j / 4], Q4, NB, true, token, 32 * b + 8 * g, x);
+                                read8(j < 4 ? tile[0] : tile[1], Q4, NB, true, 4 * gg + j % 4, 32 * b + 8 * g, x);
 #pragma unroll
                                 for (int y = 0; y < 8; ++y) {
                                     if (sees && !(__builtin_fabsf(x[y]) <= 3.402823466e38f)) acc[b][y % 2][y / 2] += pt * x[y];
@@ -301,9 +390,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn(PagedAttnArgs a) {
                 stats[wave][i][0] = m;
                 stats[wave][i][1] = l;
             }
-            __syncthreads();
+            __syncthreads();  // (and all have their queries: their place is taken)
             const int oc = static_cast<int>(threadIdx.x) / 16, od = static_cast<int>(threadIdx.x) % 16 * 8;
-            const int64_t out_c = ct * kColumns + oc;
+            const uint32_t out_c = c0 + oc, out_j = over(out_c, a.group), out_head = h * a.group.d + (out_c - out_j * a.group.d);
             float top = -__builtin_inff(), mine_top = -__builtin_inff(), sum = 0;
             for (int w = 0; w < kWaves; ++w) {
                 top = __builtin_fmaxf(top, stats[w][oc][0]);
@@ -312,7 +401,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn(PagedAttnArgs a) {
             const float base = top == -__builtin_inff() ? 0.0f : top;
             for (int w = 0; w < kWaves; ++w) sum += stats[w][oc][1] * __builtin_amdgcn_exp2f(stats[w][oc][0] - base);
             const float f = __builtin_amdgcn_exp2f(m - (mine_top == -__builtin_inff() ? 0.0f : mine_top));
-            const int64_t out_row = sr.begin + out_c / a.group, out_head = static_cast<int64_t>(h) * a.group + out_c % a.group;
+            const float inv = sum == 0 ? 0.0f : 1.0f / sum;
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
                 if (n != 0) __syncthreads();
@@ -327,24 +416,23 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn(PagedAttnArgs a) {
                         hi[2 * r] = acc[b][0][r + 2] * f;
                         hi[2 * r + 1] = acc[b][1][r + 2] * f;
                     }
-                    *reinterpret_cast<float4v*>(&merge[wave][i][32 * k + 8 * g]) = lo;
-                    *reinterpret_cast<float4v*>(&merge[wave][i][32 * k + 8 * g + 4]) = hi;
+                    *reinterpret_cast<float4v*>(&lds.merge[wave][i][32 * k + 8 * g]) = lo;
+                    *reinterpret_cast<float4v*>(&lds.merge[wave][i][32 * k + 8 * g + 4]) = hi;
                 }
                 __syncthreads();
                 if (od < 32 * GS && out_c < cols) {
                     float y[8];
                     for (int j = 0; j < 8; ++j) {
-                        y[j] = merge[0][oc][od + j];
-                        for (int w = 1; w < kWaves; ++w) y[j] += merge[w][oc][od + j];
+                        y[j] = lds.merge[0][oc][od + j];
+                        for (int w = 1; w < kWaves; ++w) y[j] += lds.merge[w][oc][od + j];
                     }
                     const int d = 128 * n + od;
                     if (a.splits == 1) {
-                        const float inv = sum == 0 ? 0.0f : 1.0f / sum;
                         for (int j = 0; j < 8; ++j) y[j] = sum == 0 ? 0.0f : y[j] * inv;
-                        char* op = row_ptr(a.out, out_row, out_head);
+                        char* op = row_ptr(a.out, sr.begin + out_j, out_head);
                         store8(op, a.out.type, (reinterpret_cast<uintptr_t>(op) & 15) == 0, d, y);
                     } else {
-                        const size_t u = (static_cast<size_t>(out_row) * a.heads + out_head) * a.splits + blockIdx.x;
+                        const size_t u = (static_cast<size_t>(sr.begin + out_j) * a.heads + out_head) * a.splits + blockIdx.x;
                         store8(a.part + u * HD, kTypeF32, true, d, y);
                         if (d == 0) {
                             float* ml = a.part + static_cast<size_t>(a.b.rows) * a.heads * a.splits * HD + u * 2;
@@ -354,34 +442,61 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn(PagedAttnArgs a) {
                     }
                 }
             }
-            __syncthreads();  // the next columns' statistics
+            __syncthreads();  // the next columns' queries and statistics
         }
     }
 }
 
-// Joins the parts of a row's head, in their order: one wave each.
+// Joins the parts of a row's head, in their order: a workgroup each.  Its threads weigh the parts once,
+// then each group of HD / 4 threads adds every 1024 / HD-th part.
+constexpr uint32_t kMaxSplits = 256;
 __global__ __launch_bounds__(256) void k_paged_join(PagedAttnArgs a) {
-    const int lane = static_cast<int>(threadIdx.x) % 64, wave = static_cast<int>(threadIdx.x) / 64, hd = static_cast<int>(a.kv.head_dim);
-    const float* stats = a.part + static_cast<size_t>(a.b.rows) * a.heads * a.splits * hd;
+    __shared__ float weight[kMaxSplits], red[4];
+    __shared__ float4v sums[256];
+    const uint32_t t = threadIdx.x, hd = a.kv.head_dim, quads = hd / 4, groups = 256 / quads, splits = a.splits;
+    const float* stats = a.part + static_cast<size_t>(a.b.rows) * a.heads * splits * hd;
     for (uint32_t s = blockIdx.y; s < a.b.seqs; s += gridDim.y) {
         const SeqRows sr = seq_rows(a.b, s);
-        const int64_t total = (sr.end - sr.begin) * a.heads;
-        for (int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + wave; u < total; u += static_cast<int64_t>(gridDim.x) * 4) {
-            const int64_t row = sr.begin + u / a.heads, head = u % a.heads;
-            const size_t at = (static_cast<size_t>(row) * a.heads + head) * a.splits;
-            float top = -__builtin_inff();
-            for (uint32_t p = 0; p < a.splits; ++p) top = __builtin_fmaxf(top, stats[(at + p) * 2]);
-            const float base = top == -__builtin_inff() ? 0.0f : top;
-            float sum = 0;
-            for (uint32_t p = 0; p < a.splits; ++p) sum += stats[(at + p) * 2 + 1] * __builtin_amdgcn_exp2f(stats[(at + p) * 2] - base);
-            for (int d = lane; d < hd; d += 64) {
-                float y = 0;
-                for (uint32_t p = 0; p < a.splits; ++p) y += a.part[(at + p) * hd + d] * __builtin_amdgcn_exp2f(stats[(at + p) * 2] - base);
-                y = sum == 0 ? 0.0f : y / sum;
-                char* op = row_ptr(a.out, row, head);
-                if (a.out.type == kTypeF32) reinterpret_cast<float*>(op)[d] = y;
-                else reinterpret_cast<uint16_t*>(op)[d] = static_cast<uint16_t>(a.out.type == kTypeF16 ? to_half(y) : to_bf16(y));
+        const uint32_t total = (sr.end - sr.begin) * a.heads;
+        for (uint32_t u = blockIdx.x; u < total; u += gridDim.x) {
+            const uint32_t row = over(u, a.per_row), head = u - row * a.heads;
+            const size_t at = (static_cast<size_t>(sr.begin + row) * a.heads + head) * splits;
+            float m = -__builtin_inff(), l = 0;
+            if (t < splits) {
+                m = stats[(at + t) * 2];
+                l = stats[(at + t) * 2 + 1];
             }
+            float top = m;
+            for (int x = 1; x < 64; x *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, x));
+            if (t % 64 == 0) red[t / 64] = top;
+            __syncthreads();
+            for (int w = 0; w < 4; ++w) top = __builtin_fmaxf(top, red[w]);
+            const float w = __builtin_amdgcn_exp2f(m - (top == -__builtin_inff() ? 0.0f : top));
+            if (t < splits) weight[t] = w;
+            float sum = t < splits ? l * w : 0.0f;
+            for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
+            __syncthreads();
+            if (t % 64 == 0) red[t / 64] = sum;
+            const uint32_t g = t / quads, d = t % quads * 4;
+            float4v y{0, 0, 0, 0};
+            if (g < groups) {
+#pragma unroll 4
+                for (uint32_t p = g; p < splits; p += groups) y += *reinterpret_cast<const float4v*>(a.part + (at + p) * hd + d) * weight[p];
+            }
+            sums[t] = y;
+            __syncthreads();
+            if (t < quads) {
+                for (uint32_t k = 1; k < groups; ++k) y += sums[k * quads + t];
+                sum = red[0] + red[1] + red[2] + red[3];
+                const float inv = 1.0f / sum;
+                char* op = row_ptr(a.out, sr.begin + row, head);
+                for (int j = 0; j < 4; ++j) {
+                    const float z = sum == 0 ? 0.0f : y[j] * inv;
+                    if (a.out.type == kTypeF32) reinterpret_cast<float*>(op)[d + j] = z;
+                    else reinterpret_cast<uint16_t*>(op)[d + j] = static_cast<uint16_t>(a.out.type == kTypeF16 ? to_half(z) : to_bf16(z));
+                }
+            }
+            __syncthreads();
         }
     }
 }
@@ -413,7 +528,7 @@ uint32_t paged_splits(const PagedKv& kv, const PagedBatch& b, uint32_t heads) {
     const uint64_t length = b.max_length == 0 ? capacity : std::min<uint64_t>(b.max_length, capacity);
     const uint64_t useful = (length + kWaves * kStep - 1) / (kWaves * kStep);
     const uint64_t wanted = (1024 + blocks - 1) / blocks;
-    return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(std::min(useful, wanted), 256)));
+    return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(std::min(useful, wanted), kMaxSplits)));
 }
 
 size_t paged_workspace(const PagedKv& kv, const PagedBatch& b, uint32_t heads) {
@@ -433,7 +548,7 @@ hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t st) {
         case 16: e = launch_sized<16>(a, grid, st); break;
     }
     if (e != hipSuccess || a.splits == 1) return e;
-    const uint64_t y = std::min<uint64_t>(a.b.seqs, 65535), x = (static_cast<uint64_t>(most_rows(a.b)) * a.heads + 3) / 4;
+    const uint64_t y = std::min<uint64_t>(a.b.seqs, 65535), x = static_cast<uint64_t>(most_rows(a.b)) * a.heads;
     const uint64_t most = std::max<uint64_t>(1, 65536 / y);
     k_paged_join<<<dim3(static_cast<uint32_t>(std::min(x, most)), static_cast<uint32_t>(y)), dim3(256), 0, st>>>(a);
     return hipGetLastError();

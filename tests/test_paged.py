@@ -147,6 +147,7 @@ def test_attention_refusals(lib):
     refused(lib, call(heads_=3), "multiple of the key/value heads")
     refused(lib, call(scale=float("inf")), "finite")
     refused(lib, call(scale=float("nan")), "finite")
+    refused(lib, call(heads_=65536, b=batch(rows=1 << 20)), "too many rows and heads")
     long = batch(page_stride=4096, max_length=60000)
     need = lib.brisk_hip_paged_attention_bytes(r(c), r(long), 4)
     assert need > 0
@@ -197,8 +198,8 @@ int main() {
     int32_t table[8] = {3, -1, 9, 0, 10, 2147483647, -2147483647, 1}, starts[5] = {0, 4, 2, 9, 40}, lengths[4] = {70, 5, -3, 100};
     PagedKv kv{nullptr, 1, 2, 64, 32, 10, 5};
     PagedBatch b{starts, lengths, table, 4, 20, 4, 0, 0};
-    const long want[][3] = {{0, 0, 3}, {0, 31, 3}, {0, 32, -1}, {0, 64, 9}, {0, 127, 0}, {0, 128, -1}, {0, -1, -1}, {1, 0, -1}, {1, 32, -1}, {1, 64, -1}, {1, 96, 1}, {1, 1L << 40, -1}};
-    for (auto& w : want) if (page_of(kv, b, (uint32_t)w[0], w[1]) != w[2]) return bad("page", w[0], w[1]);
+    const long want[][3] = {{0, 0, 3}, {0, 31, 3}, {0, 32, -1}, {0, 64, 9}, {0, 127, 0}, {0, 128, -1}, {0, -1, -1}, {1, 0, -1}, {1, 32, -1}, {1, 64, -1}, {1, 96, 1}, {1, 0x7FFFFFFF, -1}};
+    for (auto& w : want) if (page_of(kv, b, (uint32_t)w[0], (int32_t)w[1]) != w[2]) return bad("page", w[0], w[1]);
     // a page's tiles follow each other and end with the cache
     if (tile_at(kv, 9, 1, 31) + tile_bytes(true, 2) != size_t(10) * 2 * 2 * tile_bytes(true, 2)) return bad("end", 0, 0);
     if (tile_at(kv, 0, 0, 15) != 0 || tile_at(kv, 0, 0, 16) != tile_bytes(true, 2) || tile_at(kv, 0, 1, 0) != 2 * tile_bytes(true, 2)) return bad("order", 0, 0);
@@ -213,6 +214,15 @@ int main() {
     if (r.begin != 2 || r.end != 9 || r.first != -7) return bad("rows", 2, r.first);
     r = seq_rows(b, 3);
     if (r.begin != 9 || r.end != 20 || r.first != 69) return bad("rows", 3, r.first);
+    for (uint32_t d : {1u, 2u, 3u, 5u, 7u, 8u, 20u, 96u, 641u, 1024u, 65535u, 65536u}) {
+        const Divisor v = divisor(d);
+        for (uint32_t n : {0u, 1u, d - 1, d, d + 1, 7 * d - 1, 7 * d, 0x7FFFFFFFu / d * d - 1, 0x7FFFFFFFu / d * d, 0x7FFFFFFEu, 0x7FFFFFFFu})
+            if (over(n & 0x7FFFFFFF, v) != (n & 0x7FFFFFFF) / d) return bad("division", d, n);
+    }
+    starts[1] = 2147483647; lengths[0] = 2147483647;
+    r = seq_rows(b, 0);
+    if (r.begin != 0 || r.end != 20 || r.first != kMaxLength - 2147483647) return bad("rows", 5, r.first);
+    starts[1] = 4; lengths[0] = 70;
     starts[0] = -5;
     r = seq_rows(b, 0);
     if (r.begin != 0 || r.end != 4 || r.first != 66) return bad("rows", 4, r.first);
