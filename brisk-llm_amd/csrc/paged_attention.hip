@@ -16,42 +16,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kStep = 32;        // positions a wave takes at a time: two tiles
 constexpr int kColumns = 16;     // (row, head) pairs of a key/value head that share a pass
-// Probabilities are held as 2^kLift p relative to a maximum that is renewed once it is passed by
-// 2^kLazy: at most 2^15 as halves, and those of a half's smallest steps 2^-31 of the largest.
-constexpr float kLazy = 8.0f, kLift = 7.0f;
 constexpr int kMergeRow = 132;   // LDS floats a column, for 128 values: 16-byte rows, shifted over the banks
-
-__device__ inline half8v operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(half8v, word4v{a, b, c, d}); }
-__device__ inline float4v mfma(half8v a, half8v b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-__device__ inline uint32_t bits(half2v x) { return __builtin_bit_cast(uint32_t, x); }
-__device__ inline half2v halves(uint32_t x) { return __builtin_bit_cast(half2v, x); }
-
-// Codes less 8 of nibbles 0 and 4 (of 1 and 5, when `high`) of a word: a code in the low bits of a
-// half's significand is 1024 + n, four bits up it is 64 + n; taking the rest off is exact.
-__device__ inline half2v codes(uint32_t w, bool high) {
-    return high ? halves((w & 0x00F000F0) | 0x54005400) - half2v{72, 72} : halves((w & 0x000F000F) | 0x64006400) - half2v{1032, 1032};
-}
-
-// Whether halves of a word are infinities or NaN, or as 4-bit scales past kMaxScale: then bit 15 or 31 of the
-// result is set, by the carry out of the exponent (exponents of 31 all ones, of 28 on for a scale).
-template <bool SCALE>
-__device__ inline uint32_t ill(uint32_t w) { return (w & 0x7FFF7FFF) + (SCALE ? 0x10001000 : 0x04000400); }
-constexpr uint32_t kIll = 0x80008000;
-template <bool SCALE>
-__device__ inline uint32_t without_ill(uint32_t w) {
-    const uint32_t x = ill<SCALE>(w);
-    return w & ((x & 0x8000 ? 0 : 0xFFFF) | (x & 0x80000000 ? 0 : 0xFFFF0000));
-}
-
-template <int N>
-struct alignas(N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4) Words {
-    uint32_t w[N];
-};
-template <int N>
-__device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {
-    const Words<N> x = *reinterpret_cast<const Words<N>*>(p);
-    for (int k = 0; k < N; ++k) w[k] = x.w[k];
-}
 
 // What a wave holds of two tiles: keys, values and, of 4-bit tiles, their scales.
 template <int NB, bool Q4>
@@ -104,7 +69,7 @@ struct TilePair {
             }
         }
     }
-    // Infinities and NaN among a group of blocks' values, and the values without them.
+    // Whether infinities or NaN are among a group of blocks' values.
     __device__ inline bool any_ill(int n) const {
         uint32_t found = 0;
         for (int x = 0; x < 2; ++x) {
@@ -116,16 +81,6 @@ struct TilePair {
             }
         }
         return __any((found & kIll) != 0);
-    }
-    __device__ inline void drop_ill(int n) {
-        for (int x = 0; x < 2; ++x) {
-            if constexpr (Q4) {
-                for (int j = 0; j < 2 * GS; ++j) vs[x][n][j] = without_ill<true>(vs[x][n][j]);
-            } else {
-                for (int r = 0; r < 4; ++r)
-                    for (int j = 0; j < GS; ++j) v[x][n][r][j] = without_ill<false>(v[x][n][r][j]);
-            }
-        }
     }
 };
 
@@ -289,7 +244,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(NB 
                     top = __builtin_fmaxf(top, __shfl_xor(top, 16));
                     top = __builtin_fmaxf(top, __shfl_xor(top, 32));
                     const float next = __builtin_fmaxf(m, top);
-                    const float f = __builtin_amdgcn_exp2f(m - (next == -__builtin_inff() ? 0.0f : next));
+                    const float f = weight(m, next);
                     m = next;
                     l *= f;
 #pragma unroll
@@ -307,7 +262,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(NB 
                     ph[j] = static_cast<_Float16>(p[j]);
                     if constexpr (EXACT) pl[j] = static_cast<_Float16>(p[j] - static_cast<float>(ph[j]));
                 }
-                bool poison = false;
 #pragma unroll
                 for (int n = 0; n < NG; ++n) {
                     if constexpr (!kEarly) {
@@ -315,13 +269,42 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(NB 
                         kv.load_values(tile[1], 1, n, lane);
                     }
                     if (!full) kv.keep_seen(n, anyones);
-                    // a value that is not finite, at a position that some column does not see: the product is
-                    // taken without it, and the columns that see it get it afterwards (4-bit: its whole block is
-                    // NaN).  With 32-bit results everywhere: an infinity times a probability's second part is of any sign
-                    if (!full || (EXACT && !Q4)) {
-                        if (kv.any_ill(n)) {
-                            kv.drop_ill(n);
-                            poison = true;
+                    // (in 4 bits a whole block is NaN, which only columns that do not see it need kept from)
+                    if ((!full || !Q4) && __builtin_expect(kv.any_ill(n), 0)) {
+                        half8v sees;
+                        for (int j = 0; j < 8; ++j) sees[j] = static_cast<_Float16>(seen >> j & 1 ? 1.0f : 0.0f);
+#pragma unroll
+                        for (int k = 0; k < GS; ++k) {
+                            const int b = n * GS + k;
+                            uint32_t up[2][4], down[2][4];  // of the lane's two columns
+                            for (int x = 0; x < 2; ++x) {
+                                if constexpr (Q4) {
+                                    for (int j = 0; j < 2; ++j) {
+                                        const Marks mk = scale_marks(kv.vs[x][n][2 * k + j]);
+                                        kv.vs[x][n][2 * k + j] = mk.rest;
+                                        up[0][2 * x + j] = up[1][2 * x + j] = mk.up;
+                                        down[0][2 * x + j] = down[1][2 * x + j] = mk.down;
+                                    }
+                                } else {
+                                    for (int j = 0; j < 2; ++j) {
+                                        const Marks m0 = marks(kv.v[x][n][2 * j][k]), m1 = marks(kv.v[x][n][2 * j + 1][k]);
+                                        kv.v[x][n][2 * j][k] = m0.rest;
+                                        kv.v[x][n][2 * j + 1][k] = m1.rest;
+                                        for (int c2 = 0; c2 < 2; ++c2) {
+                                            const uint32_t sel = c2 ? 0x07060302 : 0x05040100;
+                                            up[c2][2 * x + j] = __builtin_amdgcn_perm(m1.up, m0.up, sel);
+                                            down[c2][2 * x + j] = __builtin_amdgcn_perm(m1.down, m0.down, sel);
+                                        }
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int c2 = 0; c2 < 2; ++c2) {
+                                const float4v none{0, 0, 0, 0};
+                                const float4v u = mfma(operand(up[c2][0], up[c2][1], up[c2][2], up[c2][3]), sees, none);
+                                const float4v d = mfma(operand(down[c2][0], down[c2][1], down[c2][2], down[c2][3]), sees, none);
+                                for (int r = 0; r < 4; ++r) acc[b][c2][r] += ill_sum(u[r], d[r]);
+                            }
                         }
                     }
 #pragma unroll
@@ -359,28 +342,6 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(NB 
                         }
                     }
                 }
-                if (__builtin_expect(poison, 0)) {
-#pragma unroll 1
-                    for (int j = 0; j < 8; ++j) {
-#pragma unroll 1
-                        for (int gg = 0; gg < 4; ++gg) {
-                            float pt = 0;
-#pragma unroll
-                            for (int y = 0; y < 8; ++y) pt = y == j ? p[y] : pt;
-                            pt = __shfl(pt, i + 16 * gg);
-                            const bool sees = __shfl(seen, i + 16 * gg) >> j & 1;
-#pragma unroll
-                            for (int b = 0; b < NB; ++b) {
-                                float x[8];
-                                read8(j < 4 ? tile[0] : tile[1], Q4, NB, true, 4 * gg + j % 4, 32 * b + 8 * g, x);
-#pragma unroll
-                                for (int y = 0; y < 8; ++y) {
-                                    if (sees && !(__builtin_fabsf(x[y]) <= 3.402823466e38f)) acc[b][y % 2][y / 2] += pt * x[y];
-                                }
-                            }
-                        }
-                    }
-                }
             }
             l += __shfl_xor(l, 16);
             l += __shfl_xor(l, 32);
@@ -398,9 +359,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(NB 
                 top = __builtin_fmaxf(top, stats[w][oc][0]);
                 mine_top = __builtin_fmaxf(mine_top, stats[w][i][0]);
             }
-            const float base = top == -__builtin_inff() ? 0.0f : top;
-            for (int w = 0; w < kWaves; ++w) sum += stats[w][oc][1] * __builtin_amdgcn_exp2f(stats[w][oc][0] - base);
-            const float f = __builtin_amdgcn_exp2f(m - (mine_top == -__builtin_inff() ? 0.0f : mine_top));
+            for (int w = 0; w < kWaves; ++w) sum += stats[w][oc][1] * weight(stats[w][oc][0], top);
+            const float f = weight(m, mine_top);
             const float inv = sum == 0 ? 0.0f : 1.0f / sum;
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
@@ -451,7 +411,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(NB 
 // then each group of HD / 4 threads adds every 1024 / HD-th part.
 constexpr uint32_t kMaxSplits = 256;
 __global__ __launch_bounds__(256) void k_paged_join(PagedAttnArgs a) {
-    __shared__ float weight[kMaxSplits], red[4];
+    __shared__ float weights[kMaxSplits], red[4];
     __shared__ float4v sums[256];
     const uint32_t t = threadIdx.x, hd = a.kv.head_dim, quads = hd / 4, groups = 256 / quads, splits = a.splits;
     const float* stats = a.part + static_cast<size_t>(a.b.rows) * a.heads * splits * hd;
@@ -471,8 +431,8 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttnArgs a) {
             if (t % 64 == 0) red[t / 64] = top;
             __syncthreads();
             for (int w = 0; w < 4; ++w) top = __builtin_fmaxf(top, red[w]);
-            const float w = __builtin_amdgcn_exp2f(m - (top == -__builtin_inff() ? 0.0f : top));
-            if (t < splits) weight[t] = w;
+            const float w = weight(m, top);
+            if (t < splits) weights[t] = w;
             float sum = t < splits ? l * w : 0.0f;
             for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
             __syncthreads();
@@ -481,7 +441,7 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttnArgs a) {
             float4v y{0, 0, 0, 0};
             if (g < groups) {
 #pragma unroll 4
-                for (uint32_t p = g; p < splits; p += groups) y += *reinterpret_cast<const float4v*>(a.part + (at + p) * hd + d) * weight[p];
+                for (uint32_t p = g; p < splits; p += groups) y += *reinterpret_cast<const float4v*>(a.part + (at + p) * hd + d) * weights[p];
             }
             sums[t] = y;
             __syncthreads();
@@ -522,25 +482,34 @@ hipError_t launch_sized(const PagedAttnArgs& a, dim3 grid, hipStream_t st) {
 
 }  // namespace
 
-uint32_t paged_splits(const PagedKv& kv, const PagedBatch& b, uint32_t heads) {
-    const uint64_t blocks = static_cast<uint64_t>(b.seqs) * kv.kv_heads * column_tiles(kv, b, heads);
+// Prompts go to the kernel of many columns once those of a sequence fill half of its workgroup.
+bool is_prompt(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bool exact) {
+    return !exact && kv.head_dim <= 256 && static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads) * 2 >= prompt_columns(kv.head_dim);
+}
+
+uint32_t paged_splits(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bool exact) {
+    const bool prompt = is_prompt(kv, b, heads, exact);
+    const uint64_t wide = prompt_columns(kv.head_dim), cols = static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads);
+    const uint64_t blocks = static_cast<uint64_t>(b.seqs) * kv.kv_heads * (prompt ? (cols + wide - 1) / wide : column_tiles(kv, b, heads));
     const uint64_t capacity = static_cast<uint64_t>(b.page_stride) * kv.page_tokens;
     const uint64_t length = b.max_length == 0 ? capacity : std::min<uint64_t>(b.max_length, capacity);
-    const uint64_t useful = (length + kWaves * kStep - 1) / (kWaves * kStep);
-    const uint64_t wanted = (1024 + blocks - 1) / blocks;
+    const uint64_t least = prompt ? 512 : kWaves * kStep, useful = (length + least - 1) / least;
+    const uint64_t wanted = prompt ? 256 / blocks : (1024 + blocks - 1) / blocks;
     return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(std::min(useful, wanted), kMaxSplits)));
 }
 
 size_t paged_workspace(const PagedKv& kv, const PagedBatch& b, uint32_t heads) {
-    const size_t splits = paged_splits(kv, b, heads);
+    const size_t splits = std::max(paged_splits(kv, b, heads, false), paged_splits(kv, b, heads, true));
     return splits == 1 ? 0 : static_cast<size_t>(b.rows) * heads * splits * (kv.head_dim + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t st) {
+    const bool exact = a.q.type == kTypeF32 || a.out.type == kTypeF32, prompt = is_prompt(a.kv, a.b, a.heads, exact);
     const uint64_t tiles = std::min<uint64_t>(column_tiles(a.kv, a.b, a.heads), 65535 / a.kv.kv_heads);
     const dim3 grid(a.splits, static_cast<uint32_t>(tiles * a.kv.kv_heads), std::min<uint32_t>(a.b.seqs, 65535));
     hipError_t e = hipErrorInvalidValue;
-    switch (a.kv.head_dim / 32) {
+    if (prompt) e = launch_paged_prompt(a, most_rows(a.b), st);
+    else switch (a.kv.head_dim / 32) {
         case 2: e = launch_sized<2>(a, grid, st); break;
         case 3: e = launch_sized<3>(a, grid, st); break;
         case 4: e = launch_sized<4>(a, grid, st); break;

@@ -8,6 +8,7 @@ namespace bh {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
 typedef uint32_t word2v __attribute__((ext_vector_type(2)));
 typedef uint32_t word4v __attribute__((ext_vector_type(4)));
 
@@ -71,6 +72,59 @@ __device__ inline void store8(void* head, int type, bool vec, int d, const float
     } else {
         for (int j = 0; j < 8; ++j) p[j] = static_cast<uint16_t>(u[j]);
     }
+}
+
+// Probabilities are held as 2^kLift p relative to a maximum that is renewed once it is passed by
+// 2^kLazy: at most 2^15 as halves, and those of a half's smallest steps 2^-31 of the largest.
+constexpr float kLazy = 8.0f, kLift = 7.0f;
+
+// The factor of sums relative to maximum m once it is `next`.  Never 0, so that an infinity stays one.
+__device__ inline float weight(float m, float next) {
+    return __builtin_fmaxf(__builtin_amdgcn_exp2f(m - (next == -__builtin_inff() ? 0.0f : next)), 1.17549435e-38f);
+}
+
+__device__ inline half8v operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(half8v, word4v{a, b, c, d}); }
+__device__ inline float4v mfma(half8v a, half8v b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ inline float16v mfma(half8v a, half8v b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ inline uint32_t bits(half2v x) { return __builtin_bit_cast(uint32_t, x); }
+__device__ inline half2v halves(uint32_t x) { return __builtin_bit_cast(half2v, x); }
+
+// Codes less 8 of nibbles 0 and 4 (of 1 and 5, when `high`) of a word: a code in the low bits of a
+// half's significand is 1024 + n, four bits up it is 64 + n; taking the rest off is exact.
+__device__ inline half2v codes(uint32_t w, bool high) {
+    return high ? halves((w & 0x00F000F0) | 0x54005400) - half2v{72, 72} : halves((w & 0x000F000F) | 0x64006400) - half2v{1032, 1032};
+}
+
+// Whether halves of a word are infinities or NaN, or as 4-bit scales past kMaxScale: then bit 15 or 31 of the
+// result is set, by the carry out of the exponent (exponents of 31 all ones, of 28 on for a scale).
+template <bool SCALE>
+__device__ inline uint32_t ill(uint32_t w) { return (w & 0x7FFF7FFF) + (SCALE ? 0x10001000 : 0x04000400); }
+constexpr uint32_t kIll = 0x80008000;
+// Values that are not finite are kept out of a product, where a probability of 0 (a position that a column does not
+// see, or one rounded to 0) would make them NaN, and added by two products of marks against 1 for each
+// position a column sees: 32768 for an infinity or NaN, and for a minus infinity or NaN.
+struct Marks {
+    uint32_t up, down, rest;  // two halves each
+};
+__device__ inline Marks marks(uint32_t w) {
+    const uint32_t i = ill<false>(w) & kIll, sign = w & kIll, nan = (((w & 0x03FF03FF) + 0x03FF03FF) & 0x04000400) << 5;
+    return {((i & (~sign | nan)) >> 15) * 0x7800, ((i & (sign | nan)) >> 15) * 0x7800, w & ~((i >> 15) * 0xFFFF)};
+}
+// (each product is rounded, to an infinity or 0: a fused one would not be)
+__device__ inline float ill_sum(float up, float down) { return up * 3e38f - down * 3e38f; }
+__device__ inline Marks scale_marks(uint32_t w) {  // blocks without a scale are NaN
+    const uint32_t i = (ill<true>(w) & kIll) >> 15;
+    return {i * 0x7800, i * 0x7800, w & ~(i * 0xFFFF)};
+}
+
+template <int N>
+struct alignas(N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4) Words {
+    uint32_t w[N];
+};
+template <int N>
+__device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+    const Words<N> x = *reinterpret_cast<const Words<N>*>(p);
+    for (int k = 0; k < N; ++k) w[k] = x.w[k];
 }
 
 // Eight values of a position of a tile, from dimension d (a multiple of 8) on.

@@ -51,11 +51,12 @@ def held(x, kind):
 
 def attend(q, k, v, positions, held_at, scale, window):
     """One sequence: q [rows, heads, dim], k and v [length, kv_heads, dim] in 64 bits, the rows' positions, and which cached
-    positions there are.  Returns the outputs, sum p |v|, the largest sum |q| |k| scale of each row's head, and sum |v|."""
+    positions there are.  Returns the outputs, sum p |v|, the largest sum |q| |k| scale of each row's head, sum |v|, and the
+    largest root of sum (q k scale)^2."""
     rows, heads, dim = q.shape
     group = heads // k.shape[1]
     t = np.arange(k.shape[0])
-    out, mass, size, total = (np.zeros((rows, heads, n)) for n in (dim, dim, 1, dim))
+    out, mass, size, total, spread = (np.zeros((rows, heads, n)) for n in (dim, dim, 1, dim, 1))
     for r in range(rows):
         see = held_at & (t <= positions[r])
         if window:
@@ -73,8 +74,9 @@ def attend(q, k, v, positions, held_at, scale, window):
                 out[r, h] = (p[:, None] * vv).sum(0)
                 mass[r, h] = (p[:, None] * np.abs(vv)).sum(0)
                 total[r, h] = np.abs(vv).sum(0)
+                spread[r, h] = np.sqrt(((kk * q[r, h]) ** 2).sum(1).max()) * abs(scale)
                 size[r, h] = (np.abs(kk) @ np.abs(q[r, h])).max() * abs(scale)
-    return out, mass, size, total
+    return out, mass, size, total, spread
 
 
 class Batch:

@@ -7,7 +7,9 @@ exact products summed in 32 bits with at most dim / 8 roundings on a path, by e 
 probability by at most 2 e of it, as the exponential's own error (2^-21) does; the sums over L positions add L / 16 + 32 roundings of
 2^-24.  In 32 bits the queries and probabilities are sums of two 16-bit parts: 2^-21 in the place of 2^-10, and twice
 the score's terms, with 2^-21 of sum |q| |k| scale for the query's own remainder.  A probability next to 0 is held in a half's smallest
-steps, 2^-24 where the largest is at least 2^7: off by half a step, 2^-32 of the largest, which is at most 1, so 2^-32 sum |v| in all.
+steps, 2^-24 where the largest is at least 2^7: off by half a step, 2^-32 of the largest, which is at most 1, so 2^-32 sum |v| in all.  Prompts' 4-bit
+keys are rounded to 16 bits as their values are, each by at most 2^-11 of it and independently: by Hoeffding's bound a score is off by
+more than 7.5 2^-11 sqrt(sum (q k scale)^2) once in 10^12.
 """
 import ctypes as C
 
@@ -297,9 +299,11 @@ def check_attention(cache, q, out, scale, window, kv=None):
     for s, (r, l) in enumerate(zip(b.rows, b.lengths)):
         mine = slice(b.starts[s], b.starts[s] + r)
         at = slice(starts[s], starts[s] + max(l, 0))
-        want, mass, size, total = R.attend(qq[mine], k[at], v[at], np.arange(l - r, l), there[s], float(np.float32(scale)), window)
+        want, mass, size, total, spread = R.attend(qq[mine], k[at], v[at], np.arange(l - r, l), there[s], float(np.float32(scale)), window)
         dim = q.shape[2]
         score = (dim / 8 * (2 if exact else 1) * 2.0 ** -24 + (2.0 ** -21 if exact else 0)) * size
+        if cache.kind == Q4_0 and not exact and r > 8:
+            score = score + 7.5 * 2.0 ** -11 * spread
         tol = HALF_STEP[kind] * np.abs(want) + mass * ((2.0 ** -21 if exact else 2.0 ** -10) + 2 * score + 2.0 ** -20 + (l / 16 + 32) * 2.0 ** -24) + 2.0 ** -32 * total
         fine = np.isfinite(want)
         assert (np.isnan(got[mine]) == np.isnan(want)).all(), f"sequence {s}: NaN"
@@ -326,10 +330,10 @@ def filled(lib, batch, kind, kvh, dim, seed=0, **more):
     return cache
 
 
-LENGTHS = [([1, 1, 1, 1], [1, 17, 700, 1300]), ([3, 8, 1], [40, 8, 333]), ([70, 33], [200, 33])]
+LENGTHS = [([1, 1, 1, 1], [1, 17, 700, 1300]), ([3, 8, 1], [40, 8, 333]), ([70, 33], [200, 33]), ([300, 1, 0, 129], [300, 500, 70, 700])]
 
 
-@pytest.mark.parametrize("rows_,lengths", LENGTHS, ids=["tokens", "drafted", "prompts"])
+@pytest.mark.parametrize("rows_,lengths", LENGTHS, ids=["tokens", "drafted", "prompts", "mixed"])
 @pytest.mark.parametrize("kind", [F16, Q4_0], ids=NAMES.get)
 @pytest.mark.parametrize("heads,kvh,dim,src", [(16, 8, 128, F16), (4, 1, 64, BF16), (6, 2, 96, F32), (4, 1, 256, F32), (8, 2, 256, F16), (8, 1, 512, F32),
                                                (8, 1, 512, BF16), (20, 5, 128, F32), (32, 1, 64, F16), (3, 3, 128, BF16)])
@@ -423,6 +427,27 @@ def test_attention_values_that_are_not_finite(lib, kind, src, rows_, window):
     if window:  # without one, position 45 is seen
         assert np.isfinite(got[-6]).all()
     assert not np.isfinite(got[-1]).any()  # a NaN key: its row's every value
+
+
+@pytest.mark.parametrize("src", [F16, F32], ids=NAMES.get)
+@pytest.mark.parametrize("rows_", [1, 200])
+def test_attention_infinity_with_a_small_probability(lib, src, rows_):
+    """A probability that rounds to 0 times an infinite value: the infinity, as in the formula."""
+    batch = Batch([rows_], [300], 16)
+    cache = Cache(lib, batch, F16, 1, 64, max_rows=0)
+    k, v = np.zeros((300, 1, 64), np.float32), np.ones((300, 1, 64), np.float32)
+    k[0], k[1:] = 1, -1
+    v[5, 0, 2], v[6, 0, 3] = np.inf, -np.inf
+    every = Batch([300], [300], 16)
+    every.table, every.pages = batch.table, batch.pages
+    cache.set(every)
+    cache.append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+    cache.set(batch)
+    q = torch.ones(rows_, 2, 64, dtype=TORCH[src], device="cuda")
+    got = host(cache.attend(q, 0.35))  # scores of 22.4 and -22.4
+    assert (got[:, :, 2] == np.inf).all() and (got[:, :, 3] == -np.inf).all()
+    rest = np.delete(got, [2, 3], axis=2)
+    assert (np.abs(rest - 1) <= 2.0 ** -9).all()
 
 
 def test_attention_queries_that_are_not_finite_or_extreme(lib):
@@ -542,10 +567,10 @@ def test_serving_steps_eager_and_captured(lib, kind):
             k, _ = R.held(R.norm_rope(rows_[:, heads:heads + kvh], host(w[1]), eps, table, pos, dim, 1), kind)
             v, _ = R.held(rows_[:, heads + kvh:].astype(np.float64), kind)
             q = R.norm_rope(rows_[-b.rows[s]:, :heads], host(w[0]), eps, table, pos[-b.rows[s]:], dim, 1)
-            want, mass, size, _ = R.attend(q, k, v, pos[-b.rows[s]:], np.ones(len(pos), bool), scale, 0)
+            want, mass, size, _, spread = R.attend(q, k, v, pos[-b.rows[s]:], np.ones(len(pos), bool), scale, 0)
             # queries and (16-bit) keys are rounded to 16 bits: 2^-11 of sum |q| |k| scale each, in a score; the cached keys are the same but
             # for those that the norm's last place moves over a border: none of these seeds' values is
-            tol = mass * (2 * (2 * 2.0 ** -11) * size + 2.0 ** -19)
+            tol = mass * (2 * (2 * 2.0 ** -11) * size + 2.0 ** -19)  # (32-bit outputs: no rounding of 4-bit products)
             assert (np.abs(got[b.starts[s]:b.starts[s + 1]] - want) <= tol).all()
 
     load(0)
