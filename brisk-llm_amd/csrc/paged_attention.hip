@@ -484,12 +484,12 @@ hipError_t launch_sized(const PagedAttnArgs& a, dim3 grid, hipStream_t st) {
 
 // Prompts go to the kernel of many columns once those of a sequence fill half of its workgroup.
 bool is_prompt(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bool exact) {
-    return !exact && kv.head_dim <= 256 && static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads) * 2 >= prompt_columns(kv.head_dim);
+    return prompt_fits(kv.head_dim, exact) && static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads) * 2 >= prompt_columns();
 }
 
 uint32_t paged_splits(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bool exact) {
     const bool prompt = is_prompt(kv, b, heads, exact);
-    const uint64_t wide = prompt_columns(kv.head_dim), cols = static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads);
+    const uint64_t wide = prompt_columns(), cols = static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads);
     const uint64_t blocks = static_cast<uint64_t>(b.seqs) * kv.kv_heads * (prompt ? (cols + wide - 1) / wide : column_tiles(kv, b, heads));
     const uint64_t capacity = static_cast<uint64_t>(b.page_stride) * kv.page_tokens;
     const uint64_t length = b.max_length == 0 ? capacity : std::min<uint64_t>(b.max_length, capacity);
@@ -508,7 +508,7 @@ hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t st) {
     const uint64_t tiles = std::min<uint64_t>(column_tiles(a.kv, a.b, a.heads), 65535 / a.kv.kv_heads);
     const dim3 grid(a.splits, static_cast<uint32_t>(tiles * a.kv.kv_heads), std::min<uint32_t>(a.b.seqs, 65535));
     hipError_t e = hipErrorInvalidValue;
-    if (prompt) e = launch_paged_prompt(a, most_rows(a.b), st);
+    if (prompt) e = launch_paged_prompt(a, exact, most_rows(a.b), st);
     else switch (a.kv.head_dim / 32) {
         case 2: e = launch_sized<2>(a, grid, st); break;
         case 3: e = launch_sized<3>(a, grid, st); break;

@@ -13,42 +13,47 @@
 namespace bh {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kBlock = 64;  // positions in LDS at a time: a tile for each wave to unpack
-constexpr int kWide = 32;   // columns of a product
+constexpr int kWaves = 8;
+constexpr int kBlock = 64;  // positions in LDS at a time: four tiles, of each of which one wave unpacks the keys, one the values
+constexpr int kVector = 0x2, kMfma = 0x8;  // instructions' classes, for their order
+constexpr int kWide = 32;   // columns of a wave: (row, head) pairs of a key/value head
 
-// What a thread holds of its wave's tile until it goes to LDS.
+// What a thread holds of its wave's keys or values until they go to LDS.
 template <int NB, bool Q4>
 struct RawTile {
     static constexpr int GS = NB < 4 ? NB : 4, NG = NB / GS;
-    uint32_t k[NG][Q4 ? GS : 4 * GS], v[NG][Q4 ? 1 : 4][GS], vs[NG][Q4 ? 2 * GS : 1];
-    uint16_t ks[Q4 ? NB : 1];
+    uint32_t w[NG][Q4 ? 1 : 4][GS], s[NG][Q4 ? 2 * GS : 1];
 
-    __device__ inline void load(const uint8_t* tile, int lane) {
-        const uint8_t* at = tile + tile_values_at(Q4, NB);
-        const int i = lane % 16, g = lane / 16;
+    __device__ inline void load_keys(const uint8_t* tile, int lane) {
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             if constexpr (Q4) {
-                load_words<GS>(tile + (n * 64 + lane) * GS * 4, k[n]);
-                load_words<GS>(at + (n * 64 + lane) * GS * 4, v[n][0]);
-                load_words<2 * GS>(tile + tile_value_scales_at(NB) + (g * NB + n * GS) * 8, vs[n]);
+                load_words<GS>(tile + (n * 64 + lane) * GS * 4, w[n][0]);
+#pragma unroll
+                for (int e = 0; e < GS; ++e)  // the lane's position's scale, twice
+                    s[n][e] = *reinterpret_cast<const uint16_t*>(tile + scale_offset(NB, false, lane % 16, n * GS + e)) * 0x10001u;
             } else {
 #pragma unroll
-                for (int j = 0; j < GS; ++j) {
-                    const word4v w = *reinterpret_cast<const word4v*>(tile + ((n * GS + j) * 64 + lane) * 16);
-                    for (int e = 0; e < 4; ++e) k[n][4 * j + e] = w[e];
+                for (int e = 0; e < GS; ++e) {
+                    const word4v x = *reinterpret_cast<const word4v*>(tile + ((n * GS + e) * 64 + lane) * 16);
+                    for (int j = 0; j < 4; ++j) w[n][j][e] = x[j];
                 }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) load_words<GS>(at + ((r * NG + n) * 64 + lane) * GS * 4, v[n][r]);
             }
         }
-        if constexpr (Q4) {
+    }
+    __device__ inline void load_values(const uint8_t* tile, int lane) {
+        const uint8_t* at = tile + tile_values_at(Q4, NB);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) ks[b] = *reinterpret_cast<const uint16_t*>(tile + tile_key_scales_at(NB) + ((i / 4 * NB + b) * 4 + i % 4) * 2);
+        for (int n = 0; n < NG; ++n) {
+            if constexpr (Q4) {
+                load_words<GS>(at + (n * 64 + lane) * GS * 4, w[n][0]);
+                load_words<2 * GS>(tile + tile_value_scales_at(NB) + (lane / 16 * NB + n * GS) * 8, s[n]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) load_words<GS>(at + ((r * NG + n) * 64 + lane) * GS * 4, w[n][r]);
+            }
         }
     }
-
     // The values of positions 4 g + r whose bit r of `keep` is not set become zeros.
     __device__ inline void keep_values(uint32_t keep) {
 #pragma unroll
@@ -57,27 +62,27 @@ struct RawTile {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t b = keep >> (2 * j), mask = (b & 1 ? 0xFFFF : 0) | (b & 2 ? 0xFFFF0000 : 0);
-                    for (int e = 0; e < GS; ++e) vs[n][2 * e + j] &= mask;
+                    for (int e = 0; e < GS; ++e) s[n][2 * e + j] &= mask;
                 }
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const uint32_t mask = keep >> r & 1 ? 0xFFFFFFFF : 0;
-                    for (int e = 0; e < GS; ++e) v[n][r][e] &= mask;
+                    for (int e = 0; e < GS; ++e) w[n][r][e] &= mask;
                 }
             }
         }
     }
-    // Whether an infinity or NaN is among the values.
+    // Whether an infinity or NaN is among the values; and zeros in their place.
     __device__ inline bool any_ill() const {
         uint32_t found = 0;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             if constexpr (Q4) {
-                for (int e = 0; e < 2 * GS; ++e) found |= ill<true>(vs[n][e]);
+                for (int e = 0; e < 2 * GS; ++e) found |= ill<true>(s[n][e]);
             } else {
                 for (int r = 0; r < 4; ++r)
-                    for (int e = 0; e < GS; ++e) found |= ill<false>(v[n][r][e]);
+                    for (int e = 0; e < GS; ++e) found |= ill<false>(w[n][r][e]);
             }
         }
         return __any((found & kIll) != 0);
@@ -86,68 +91,84 @@ struct RawTile {
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             if constexpr (Q4) {
-                for (int e = 0; e < 2 * GS; ++e) vs[n][e] = scale_marks(vs[n][e]).rest;
+                for (int e = 0; e < 2 * GS; ++e) s[n][e] = scale_marks(s[n][e]).rest;
             } else {
                 for (int r = 0; r < 4; ++r)
-                    for (int e = 0; e < GS; ++e) v[n][r][e] = marks(v[n][r][e]).rest;
+                    for (int e = 0; e < GS; ++e) w[n][r][e] = marks(w[n][r][e]).rest;
             }
         }
     }
 };
 
-template <int NB>
+// Operands [32 positions][16 dimensions] and [32 dimensions][16 positions], 64 lanes x 16 bytes each, in one plane or,
+// for 4-bit values with 32-bit results, in two that add up to them.
+template <int NB, int PLANES>
 struct BlockLds {
-    // operands [32 positions][16 dimensions] and [32 dimensions][16 positions], 64 lanes x 16 bytes each
-    word4v k[kBlock / 32][2 * NB][64];
-    word4v v[NB][kBlock / 16][64];
-    int there[kWaves], poison[kWaves];  // whether a tile is there, and holds values that are not finite (here they are zeros)
+    word4v k[PLANES][kBlock / 32][2 * NB][64];
+    word4v v[PLANES][NB][kBlock / 16][64];
+    uint8_t there[kBlock / 16], poison[kBlock / 16];  // whether a tile is there, and holds values that are not finite (here they are zeros)
 };
 
-// Unpacks tile x of the block.  4-bit values are rounded to halves as codes times scales: 2^-11 of a
-// value at most, as the probabilities are.
-template <int NB, bool Q4>
-__device__ inline void unpack(const RawTile<NB, Q4>& raw, BlockLds<NB>& out, int x, int lane) {
+// A code times its scale, in one half (rounded: 2^-11 of the value at most, as the probabilities are), or in two (exact).
+template <int PLANES>
+__device__ inline void scaled(half2v code, uint32_t scale, uint32_t (&out)[PLANES]) {
+    const half2v d = halves(scale), x = code * d;
+    out[0] = bits(x);
+    if constexpr (PLANES == 2) out[1] = bits(__builtin_elementwise_fma(code, d, -x));
+}
+
+template <int NB, bool Q4, int PLANES>
+__device__ inline void unpack_keys(const RawTile<NB, Q4>& raw, BlockLds<NB, PLANES>& out, int x, int lane) {
     constexpr int GS = NB < 4 ? NB : 4;
     const int i = lane % 16, g = lane / 16;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const int n = b / GS, e = b % GS;
-        word4v key;
-        if constexpr (Q4) {
-            const uint32_t w = raw.k[n][e], w8 = w >> 8;
-            const half2v d = halves(raw.ks[b] | static_cast<uint32_t>(raw.ks[b]) << 16);
-            key = word4v{bits(codes(w, false) * d), bits(codes(w, true) * d), bits(codes(w8, false) * d), bits(codes(w8, true) * d)};
-        } else {
-            key = word4v{raw.k[n][4 * e], raw.k[n][4 * e + 1], raw.k[n][4 * e + 2], raw.k[n][4 * e + 3]};
+        uint32_t y[4][PLANES];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (Q4) scaled<PLANES>(codes(raw.w[n][0][e] >> (j / 2 * 8), j % 2), raw.s[n][e], y[j]);
+            else y[j][0] = raw.w[n][j][e];
         }
-        out.k[x / 2][2 * b + g / 2][g % 2 * 32 + x % 2 * 16 + i] = key;
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) out.k[p][x / 2][2 * b + g / 2][g % 2 * 32 + x % 2 * 16 + i] = word4v{y[0][p], y[1][p], y[2][p], y[3][p]};
+    }
+}
+
+template <int NB, bool Q4, int PLANES>
+__device__ inline void unpack_values(const RawTile<NB, Q4>& raw, BlockLds<NB, PLANES>& out, int x, int lane) {
+    constexpr int GS = NB < 4 ? NB : 4;
+    const int i = lane % 16, g = lane / 16;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int n = b / GS, e = b % GS;
 #pragma unroll
         for (int c2 = 0; c2 < 2; ++c2) {
-            word2v val;
-            if constexpr (Q4) {
-                const uint32_t w = raw.v[n][0][e];
-                val[0] = bits(codes(w, c2) * halves(raw.vs[n][2 * e]));
-                val[1] = bits(codes(w >> 8, c2) * halves(raw.vs[n][2 * e + 1]));
-            } else {
-                const uint32_t sel = c2 ? 0x07060302 : 0x05040100;
-                val[0] = __builtin_amdgcn_perm(raw.v[n][1][e], raw.v[n][0][e], sel);
-                val[1] = __builtin_amdgcn_perm(raw.v[n][3][e], raw.v[n][2][e], sel);
+            uint32_t y[2][PLANES];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if constexpr (Q4) scaled<PLANES>(codes(raw.w[n][0][e] >> (j * 8), c2), raw.s[n][2 * e + j], y[j]);
+                else y[j][0] = __builtin_amdgcn_perm(raw.w[n][2 * j + 1][e], raw.w[n][2 * j][e], c2 ? 0x07060302 : 0x05040100);
             }
-            reinterpret_cast<word2v*>(&out.v[b][x][g % 2 * 32 + 2 * i + c2])[g / 2] = val;
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) reinterpret_cast<word2v*>(&out.v[p][b][x][g % 2 * 32 + 2 * i + c2])[g / 2] = word2v{y[0][p], y[1][p]};
         }
     }
 }
 
-// A workgroup of four waves takes CT x 128 columns, (row, head) pairs of one key/value head, each wave
-// CT x 32 of them, and one part of the positions.  Without a window a wave's two sets of columns are one from the
-// front of the prompt and its mirror image from the back: what two sets see adds up to the same for all.
-template <int NB, int CT, bool Q4>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1))) void k_paged_prompt(PagedAttnArgs a) {
-    constexpr int HD = 32 * NB;
+// A workgroup takes 256 columns and one part of the positions, a wave 32 columns.  Without a window half of the
+// waves' columns are from the front of the prompt and half are their mirror image from the back: what
+// two such waves, which share a SIMD, see adds up to the same for all.
+template <int NB, bool Q4, bool EXACT>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_paged_prompt(PagedAttnArgs a) {
+    constexpr int HD = 32 * NB, PLANES = Q4 && EXACT ? 2 : 1, PARTS = EXACT ? 2 : 1;
     __shared__ union {
-        BlockLds<NB> block[2];
-        _Float16 q[kWaves][kWide][HD + 8];
-        float out[kWaves][kWide][HD + 4];
+        BlockLds<NB, PLANES> block[2];
+        struct {
+            _Float16 part[PARTS][kWaves][16][HD + 8];  // (half of a wave's columns at a time)
+            float scale[kWaves][16];
+        } q;
+        float out[kWaves][16][HD + 4];
     } lds;
     const int lane = static_cast<int>(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int col = lane % 32, half = lane / 32;
@@ -158,38 +179,26 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1))
     for (uint32_t s = blockIdx.z; s < a.b.seqs; s += gridDim.z) {
         const SeqRows sr = seq_rows(a.b, s);
         const uint32_t cols = (sr.end - sr.begin) * a.group.d, tiles = (cols + kWide - 1) / kWide;
-        const bool mirrored = CT == 2 && window == 0;
-        const uint32_t halves_of = mirrored ? (tiles + 1) / 2 : (tiles + CT - 1) / CT;  // pairs of sets
-        for (uint32_t set = first_set; set * kWaves < halves_of; set += set_step) {
-            // the wave's columns
-            const uint32_t pair = set * kWaves + wave;
-            uint32_t tile[CT];
-            int32_t pos_lo[CT], pos_hi[CT], t_lo[CT], t_hi[CT], pos[CT];
-            const auto range = [&](uint32_t t, int32_t& plo, int32_t& phi, int32_t& tlo, int32_t& thi) {
-                const uint32_t last = std::min<uint32_t>((t + 1) * kWide, cols) - 1;
-                plo = sr.first + static_cast<int32_t>(over(t * kWide, a.group));
-                phi = sr.first + static_cast<int32_t>(over(last, a.group));
-                tlo = window != 0 && plo - window + 1 > 0 ? plo - window + 1 : 0;
-                thi = std::min(phi + 1, capacity);
-            };
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                tile[c] = mirrored && c == 1 ? tiles - 1 - pair : CT * pair * (mirrored ? 0 : 1) + (mirrored ? pair : c);
-                const bool live = pair < halves_of && tile[c] < tiles && !(c == 1 && tile[c] == tile[0]);
-                pos_lo[c] = pos_hi[c] = t_lo[c] = t_hi[c] = 0;
-                if (live) range(tile[c], pos_lo[c], pos_hi[c], t_lo[c], t_hi[c]);
-                else tile[c] = tiles;
-                const uint32_t cc = tile[c] * kWide + col;
-                pos[c] = cc < cols ? sr.first + static_cast<int32_t>(over(cc, a.group)) : pos_lo[c];
-            }
-            // the workgroup's positions: from its first set's to its last one's
-            int32_t wg_lo, wg_plo, wg_phi, wg_hi, unused_lo, unused_hi, unused;
-            {
-                const uint32_t p0 = set * kWaves, p1 = std::min(p0 + kWaves, halves_of) - 1;
-                const uint32_t front = mirrored ? p0 : CT * p0, back = mirrored ? tiles - 1 - p0 : std::min<uint32_t>(CT * p1 + CT - 1, tiles - 1);
-                range(front, wg_plo, unused, wg_lo, unused_hi);
-                range(back, unused, wg_phi, unused_lo, wg_hi);
-            }
+        const uint32_t fronts = window == 0 ? (tiles + 1) / 2 : tiles, per_set = window == 0 ? kWaves / 2 : kWaves;
+        // the positions of a column tile's rows, and those that they see
+        const auto range = [&](uint32_t t, int32_t& plo, int32_t& phi, int32_t& tlo, int32_t& thi) {
+            const uint32_t last = std::min<uint32_t>((t + 1) * kWide, cols) - 1;
+            plo = sr.first + static_cast<int32_t>(over(t * kWide, a.group));
+            phi = sr.first + static_cast<int32_t>(over(last, a.group));
+            tlo = window != 0 && plo - window + 1 > 0 ? plo - window + 1 : 0;
+            thi = std::min(phi + 1, capacity);
+        };
+        for (uint32_t set = first_set; set * per_set < fronts; set += set_step) {
+            const uint32_t front = set * per_set, back_last = std::min(front + per_set, fronts) - 1;
+            uint32_t tile = front + (wave & (per_set - 1));
+            if (window == 0 && wave >= kWaves / 2) tile = tile < fronts && tiles - 1 - tile >= fronts ? tiles - 1 - tile : tiles;
+            else if (tile >= fronts) tile = tiles;
+            int32_t pos_lo = 0, pos_hi = 0, t_lo = 0, t_hi = 0;
+            if (tile < tiles) range(tile, pos_lo, pos_hi, t_lo, t_hi);
+            const int32_t pos = tile * kWide + col < cols ? sr.first + static_cast<int32_t>(over(tile * kWide + col, a.group)) : pos_lo;
+            int32_t wg_lo, wg_plo, wg_phi, wg_hi, x0, x1, x2;  // the workgroup's, from its first tile's to its last one's
+            range(front, wg_plo, x0, wg_lo, x1);
+            range(window == 0 ? tiles - 1 - front : back_last, x0, wg_phi, x2, wg_hi);
             const int32_t blk_lo = wg_lo / kBlock, blocks = wg_hi > wg_lo ? (wg_hi + kBlock - 1) / kBlock - blk_lo : 0;
             const int32_t per = (blocks + static_cast<int32_t>(a.splits) - 1) / static_cast<int32_t>(a.splits);
             const int32_t blk_begin = blk_lo + static_cast<int32_t>(std::min<int64_t>(blocks, static_cast<int64_t>(per) * split));
@@ -197,42 +206,47 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1))
 
             RawTile<NB, Q4> raw;
             bool there = false;
+            const bool keys = wave < 4;
             const auto fetch = [&](int32_t blk) {
-                const int32_t t = blk * kBlock + 16 * wave, page = page_of(a.kv, a.b, s, t);
+                const int32_t t = blk * kBlock + 16 * (wave & 3), page = page_of(a.kv, a.b, s, t);
                 there = page >= 0;
-                raw.load(a.kv.data + tile_at(a.kv, there ? page : 0, h, t), lane);
+                const uint8_t* from = a.kv.data + tile_at(a.kv, there ? page : 0, h, t);
+                if (keys) raw.load_keys(from, lane);
+                else raw.load_values(from, lane);
             };
             const auto put = [&](int32_t blk) {
-                const int32_t t = blk * kBlock + 16 * wave + 4 * (lane / 16);
+                BlockLds<NB, PLANES>& out = lds.block[blk & 1];
+                if (keys) {
+                    unpack_keys<NB, Q4, PLANES>(raw, out, wave, lane);
+                    if (lane == 0) out.there[wave] = there;
+                    return;
+                }
                 // some column does not see all of the block: what none sees is left out
                 if (!there || (blk + 1) * kBlock - 1 > wg_plo || (window != 0 && blk * kBlock <= wg_phi - window)) {
+                    const int32_t t = blk * kBlock + 16 * (wave & 3) + 4 * (lane / 16);
                     uint32_t keep = 0;
                     for (int r = 0; r < 4; ++r) keep |= there && t + r >= wg_lo && t + r <= wg_phi ? 1u << r : 0;
                     raw.keep_values(keep);
                 }
                 const bool poison = raw.any_ill();
                 if (__builtin_expect(poison, 0)) raw.drop_ill();
-                BlockLds<NB>& out = lds.block[blk & 1];
-                unpack<NB, Q4>(raw, out, wave, lane);
-                if (lane == 0) {
-                    out.there[wave] = there;
-                    out.poison[wave] = poison;
-                }
+                unpack_values<NB, Q4, PLANES>(raw, out, wave & 3, lane);
+                if (lane == 0) out.poison[wave & 3] = poison;
             };
             if (blk_begin < blk_end) fetch(blk_begin);
 
             // the columns' queries, through the wave's part of LDS: 16 lanes a column, scaled by a power of two where the
-            // type has more range than a half
+            // type has more range than a half, and by the sign of the score's scale
             __syncthreads();  // the blocks of the columns before
-            half8v q[CT][2 * NB];
-            float qscale[CT];
-#pragma unroll
-            for (int c = 0; c < CT; ++c) {
+            half8v q[PARTS][2 * NB];
+            float qscale = 0;
+#pragma unroll 1
+            for (int c0 = 0; c0 < kWide; c0 += 16) {
                 const int sub = lane % 16;
 #pragma unroll 1
-                for (int r = lane / 16; r < kWide; r += 4) {
+                for (int r = lane / 16; r < 16; r += 4) {
                     constexpr int K = (HD + 127) / 128;
-                    const uint32_t cc = tile[c] * kWide + r;
+                    const uint32_t cc = tile * kWide + c0 + r;
                     const bool live = cc < cols;
                     const uint32_t row = live ? over(cc, a.group) : 0;
                     const char* qp = row_ptr(a.q, sr.begin + row, h * a.group.d + (live ? cc - row * a.group.d : 0));
@@ -249,97 +263,164 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1))
 #pragma unroll
                     for (int k = 0; k < K; ++k) {
                         const int d = (k * 16 + sub) * 8;
-                        half8v y;
-                        for (int j = 0; j < 8; ++j) y[j] = static_cast<_Float16>(__builtin_ldexpf(x[k][j], 9 - e));
-                        if (d < HD) *reinterpret_cast<half8v*>(&lds.q[wave][r][d]) = y;
+                        half8v hi, lo;
+                        for (int j = 0; j < 8; ++j) {
+                            const float y = __builtin_ldexpf(a.scale < 0 ? -x[k][j] : x[k][j], 9 - e);
+                            hi[j] = static_cast<_Float16>(y);
+                            lo[j] = static_cast<_Float16>(y - static_cast<float>(hi[j]));
+                        }
+                        if (d < HD) {
+                            *reinterpret_cast<half8v*>(&lds.q.part[0][wave][r][d]) = hi;
+                            if constexpr (EXACT) *reinterpret_cast<half8v*>(&lds.q.part[1][wave][r][d]) = lo;
+                        }
                     }
-                    if (sub == 0) *reinterpret_cast<float*>(&lds.q[wave][r][HD]) = __builtin_ldexpf(a.scale * 1.44269504088896f, e - 9);
+                    if (sub == 0) lds.q.scale[wave][r] = __builtin_ldexpf(__builtin_fabsf(a.scale) * 1.44269504088896f, e - 9);
                 }
+                __builtin_amdgcn_wave_barrier();
+                if (col / 16 == c0 / 16) {
 #pragma unroll
-                for (int k = 0; k < 2 * NB; ++k) q[c][k] = *reinterpret_cast<const half8v*>(&lds.q[wave][col][16 * k + 8 * half]);
-                qscale[c] = *reinterpret_cast<const float*>(&lds.q[wave][col][HD]);
+                    for (int k = 0; k < 2 * NB; ++k)
+                        for (int e = 0; e < PARTS; ++e) q[e][k] = *reinterpret_cast<const half8v*>(&lds.q.part[e][wave][col % 16][16 * k + 8 * half]);
+                    qscale = lds.q.scale[wave][col % 16];
+                }
+                __builtin_amdgcn_wave_barrier();
             }
             __syncthreads();  // (the queries' place is taken by the blocks)
 
-            float m[CT], l[CT];
-            float16v acc[CT][NB];
+            float m = -__builtin_inff(), l = 0;
+            float16v acc[NB];
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                m[c] = -__builtin_inff();
-                l[c] = 0;
-                for (int b = 0; b < NB; ++b)
-                    for (int r = 0; r < 16; ++r) acc[c][b][r] = 0;
-            }
+            for (int b = 0; b < NB; ++b) acc[b] = float16v{};
 
-            // 32 positions from t0 on, for the sets of columns from FIRST on
-            const auto sub = [&](auto from, const BlockLds<NB>& in, int32_t t0, int tt) {
-                constexpr int FIRST = decltype(from)::value;
-                const bool here[2] = {in.there[2 * tt] != 0, in.there[2 * tt + 1] != 0};
-                const bool poison = (in.poison[2 * tt] | in.poison[2 * tt + 1]) != 0;
-                float16v sc[CT];
-                half8v p[CT][2];
-                uint32_t seen[CT];
+            // a block of 64 positions from t0 on: two products of 32 side by side, since one's steps wait for each other
+            const auto sub = [&](const BlockLds<NB, PLANES>& in, int32_t t0) {
+                const uint32_t there = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t*>(in.there));
+                const uint32_t poison = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t*>(in.poison));
+                float16v sc[2] = {};
+                // The operands of half of the steps are read ahead of the products of the other half; the
+                // barriers keep the compiler from undoing that.
+                const auto read_keys = [&](half8v (&x)[PLANES][2 * NB], int k0) {
 #pragma unroll
-                for (int c = FIRST; c < CT; ++c) sc[c] = float16v{};
+                    for (int k = 0; k < 2 * NB; ++k)
+                        for (int e = 0; e < PLANES; ++e) x[e][k] = __builtin_bit_cast(half8v, in.k[e][k % 2][k0 + k / 2][lane]);
+                };
+                const auto keys_times = [&](const half8v (&x)[PLANES][2 * NB], int k0) {
 #pragma unroll
-                for (int k = 0; k < 2 * NB; ++k) {
-                    const half8v kx = __builtin_bit_cast(half8v, in.k[tt][k][lane]);
+                    for (int k = 0; k < 2 * NB; ++k) {
+                        if constexpr (EXACT) {
+                            sc[k % 2] = mfma(x[0][k], q[1][k0 + k / 2], sc[k % 2]);
+                            if constexpr (Q4) sc[k % 2] = mfma(x[1][k], q[0][k0 + k / 2], sc[k % 2]);
+                        }
+                        sc[k % 2] = mfma(x[0][k], q[0][k0 + k / 2], sc[k % 2]);
+                    }
+                };
+                half8v ops[2][PLANES][2 * NB];
+                read_keys(ops[0], 0);
+                __builtin_amdgcn_sched_barrier(0);
+                read_keys(ops[1], NB);
+                __builtin_amdgcn_sched_barrier(0);
+                keys_times(ops[0], 0);
+                keys_times(ops[1], NB);
+                __builtin_amdgcn_sched_barrier(0);
+                // the values' operands likewise, of 32 positions at a time
+                const auto read_values = [&](half8v (&x)[PLANES][2 * NB], int u0) {
 #pragma unroll
-                    for (int c = FIRST; c < CT; ++c) sc[c] = mfma(kx, q[c][k], sc[c]);
-                }
+                    for (int u = 0; u < 2; ++u)
+                        for (int b = 0; b < NB; ++b)
+                            for (int e = 0; e < PLANES; ++e) x[e][u * NB + b] = __builtin_bit_cast(half8v, in.v[e][b][u0 + u][lane]);
+                };
+                read_values(ops[0], 0);
+                __builtin_amdgcn_sched_barrier(0);
+                // the column sees positions t0 + u with lo < u <= hi, in tiles that are there
+                const int32_t hi = pos - t0, lo = window != 0 ? hi - window : -1;
+                if (there != 0x01010101 || t0 + kBlock - 1 > pos_lo || (window != 0 && t0 <= pos_hi - window)) {
 #pragma unroll
-                for (int c = FIRST; c < CT; ++c) {
-                    const bool full = here[0] && here[1] && t0 + 31 <= pos_lo[c] && (window == 0 || t0 > pos_hi[c] - window);
-                    seen[c] = 0xFFFF;
-                    if (!full) {
-                        seen[c] = 0;
+                    for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            const int32_t t = t0 + 8 * (r / 4) + 4 * half + r % 4;
-                            if (here[r / 8] && t <= pos[c] && (window == 0 || t > pos[c] - window)) seen[c] |= 1u << r;
-                            else sc[c][r] = qscale[c] < 0 ? __builtin_inff() : -__builtin_inff();
+                            const int32_t u = 32 * tt + 8 * (r / 4) + 4 * half + r % 4;
+                            if (u > hi || u <= lo || (there >> (16 * tt + r / 8 * 8) & 1) == 0) sc[tt][r] = -__builtin_inff();
                         }
                     }
-                    float top = -__builtin_inff();
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        sc[c][r] *= qscale[c];
-                        top = __builtin_fmaxf(top, sc[c][r]);
-                    }
-                    if (__any(top > m[c] + kLazy)) {
-                        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-                        const float next = __builtin_fmaxf(m[c], top);
-                        const float f = weight(m[c], next);
-                        m[c] = next;
-                        l[c] *= f;
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) acc[c][b] *= f;
-                    }
-                    const float base = m[c] == -__builtin_inff() ? 0.0f : m[c] - kLift;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float e = __builtin_amdgcn_exp2f(sc[c][r] - base);
-                        l[c] += e;
-                        p[c][r / 8][r % 8] = static_cast<_Float16>(e);
-                    }
                 }
+                float tops[4];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const half8v vx = __builtin_bit_cast(half8v, in.v[b][2 * tt + u][lane]);
-#pragma unroll
-                        for (int c = FIRST; c < CT; ++c) acc[c][b] = mfma(vx, p[c][u], acc[c][b]);
-                    }
+                for (int x = 0; x < 4; ++x) {
+                    tops[x] = sc[x / 2][x % 2 * 8];
+                    for (int r = 1; r < 8; ++r) tops[x] = __builtin_fmaxf(tops[x], sc[x / 2][x % 2 * 8 + r]);
                 }
-                if (__builtin_expect(poison, 0)) {  // the values that are not finite, from the tiles themselves
-#pragma unroll 1
+                float top = __builtin_fmaxf(__builtin_fmaxf(tops[0], tops[1]), __builtin_fmaxf(tops[2], tops[3])) * qscale;
+                if (__any(top > m + kLazy)) {
+                    top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+                    const float next = __builtin_fmaxf(m, top);
+                    const float f = weight(m, next);
+                    m = next;
+                    l *= f;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) acc[b] *= f;
+                }
+                const float base = m == -__builtin_inff() ? 0.0f : m - kLift;
+                half8v p[PARTS][4];
+                float sums[2] = {};
+                const auto exponentials = [&](int tt) {
+#pragma unroll
+                    for (int r = 0; r < 16; r += 2) {
+                        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[tt][r], qscale, -base));
+                        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[tt][r + 1], qscale, -base));
+                        const half2v e{static_cast<_Float16>(e0), static_cast<_Float16>(e1)};
+                        p[0][2 * tt + r / 8][r % 8] = e[0];
+                        p[0][2 * tt + r / 8][r % 8 + 1] = e[1];
+                        if constexpr (EXACT) {
+                            p[1][2 * tt + r / 8][r % 8] = static_cast<_Float16>(e0 - static_cast<float>(e[0]));
+                            p[1][2 * tt + r / 8][r % 8 + 1] = static_cast<_Float16>(e1 - static_cast<float>(e[1]));
+                            sums[0] += e0;
+                            sums[1] += e1;
+                        } else {
+                            sums[r / 2 % 2] = __builtin_amdgcn_fdot2(e, half2v{1, 1}, sums[r / 2 % 2], false);  // (the sum of what is multiplied)
+                        }
+                    }
+                };
+                const auto values_times = [&](const half8v (&x)[PLANES][2 * NB], int u0) {
+#pragma unroll
                     for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            if constexpr (EXACT) {
+                                acc[b] = mfma(x[0][u * NB + b], p[1][u0 + u], acc[b]);
+                                if constexpr (Q4) acc[b] = mfma(x[1][u * NB + b], p[0][u0 + u], acc[b]);
+                            }
+                            acc[b] = mfma(x[0][u * NB + b], p[0][u0 + u], acc[b]);
+                        }
+                    }
+                };
+                exponentials(0);
+                __builtin_amdgcn_sched_barrier(0);
+                read_values(ops[1], 2);
+                __builtin_amdgcn_sched_barrier(0);
+                values_times(ops[0], 0);
+                exponentials(1);
+                if constexpr (!EXACT) {  // the second exponentials under the first products
+#pragma unroll
+                    for (int k = 0; k < 2 * NB; ++k) {
+                        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(kVector, 24 / NB, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                values_times(ops[1], 2);
+                l += sums[0] + sums[1];
+                if (__builtin_expect(poison != 0, 0)) {
+                    // the values that are not finite, from the tiles themselves
+#pragma unroll 1
+                    for (int u = 0; u < 4; ++u) {
                         const int32_t t = t0 + 16 * u, page = page_of(a.kv, a.b, s, t);
-                        const uint8_t* tile_ = a.kv.data + tile_at(a.kv, page < 0 ? 0 : page, h, t);
-                        half8v sees[CT];
-                        for (int c = FIRST; c < CT; ++c)
-                            for (int e = 0; e < 8; ++e) sees[c][e] = static_cast<_Float16>(seen[c] >> (8 * u + e) & 1 ? 1.0f : 0.0f);
+                        const uint8_t* from = a.kv.data + tile_at(a.kv, page < 0 ? 0 : page, h, t);
+                        half8v sees;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int32_t token = 16 * u + e / 4 * 8 + 4 * half + e % 4;
+                            sees[e] = static_cast<_Float16>(token <= hi && token > lo && page >= 0 ? 1.0f : 0.0f);
+                        }
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
                             uint32_t up[4] = {}, down[4] = {};
@@ -347,81 +428,58 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1))
                             for (int e = 0; e < 8; ++e) {
                                 const uint32_t token = e / 4 * 8 + 4 * half + e % 4, d = 32 * b + col;
                                 const uint32_t x = *reinterpret_cast<const uint16_t*>(
-                                    tile_ + (Q4 ? scale_offset(NB, true, token, b) : value_offset(false, NB, token, d & ~1) + (d & 1) * 2));
+                                    from + (Q4 ? scale_offset(NB, true, token, b) : value_offset(false, NB, token, d & ~1) + (d & 1) * 2));
                                 const Marks mk = Q4 ? scale_marks(x) : marks(x);
                                 up[e / 2] |= mk.up << (16 * (e % 2));
                                 down[e / 2] |= mk.down << (16 * (e % 2));
                             }
-#pragma unroll
-                            for (int c = FIRST; c < CT; ++c) {
-                                const float16v f = mfma(operand(up[0], up[1], up[2], up[3]), sees[c], float16v{});
-                                const float16v g = mfma(operand(down[0], down[1], down[2], down[3]), sees[c], float16v{});
-                                for (int r = 0; r < 16; ++r) acc[c][b][r] += ill_sum(f[r], g[r]);
-                            }
+                            const float16v f = mfma(operand(up[0], up[1], up[2], up[3]), sees, float16v{});
+                            const float16v g = mfma(operand(down[0], down[1], down[2], down[3]), sees, float16v{});
+                            for (int r = 0; r < 16; ++r) acc[b][r] += ill_sum(f[r], g[r]);
                         }
                     }
-                }
-            };
-            const auto walk = [&](auto from, int32_t begin, int32_t end) {
-                constexpr int FIRST = decltype(from)::value;
-                for (int32_t blk = begin; blk < end; ++blk) {
-                    if (blk + 1 < blk_end) fetch(blk + 1);
-                    const BlockLds<NB>& in = lds.block[blk & 1];
-#pragma unroll 1
-                    for (int tt = 0; tt < kBlock / 32; ++tt) {
-                        const int32_t t0 = blk * kBlock + 32 * tt;
-                        bool on = false;
-                        for (int c = FIRST; c < CT; ++c) on |= t0 < t_hi[c] && t0 + 32 > t_lo[c];
-                        if (on) sub(from, in, t0, tt);
-                    }
-                    if (blk + 1 < blk_end) put(blk + 1);
-                    __syncthreads();
                 }
             };
 
             if (blk_begin < blk_end) put(blk_begin);
             __syncthreads();
-            if constexpr (CT == 2) {
-                // once all of the workgroup's front sets have seen their positions, the back sets go on alone
-                int32_t both = blk_end;
-                if (mirrored) {
-                    int32_t front_lo, front_hi, x, y;
-                    range(std::min(set * kWaves + kWaves, halves_of) - 1, x, y, front_lo, front_hi);
-                    both = std::min(blk_end, std::max(blk_begin, (front_hi + kBlock - 1) / kBlock));
-                }
-                walk(std::integral_constant<int, 0>{}, blk_begin, both);
-                walk(std::integral_constant<int, 1>{}, both, blk_end);
-            } else {
-                walk(std::integral_constant<int, 0>{}, blk_begin, blk_end);
+            for (int32_t blk = blk_begin; blk < blk_end; ++blk) {
+                if (blk + 1 < blk_end) fetch(blk + 1);
+                const BlockLds<NB, PLANES>& in = lds.block[blk & 1];
+                const int32_t t0 = blk * kBlock;
+                if (t0 < t_hi && t0 + kBlock > t_lo) sub(in, t0);
+                if (blk + 1 < blk_end) put(blk + 1);
+                __syncthreads();
             }
 
             // out by way of the wave's part of LDS, so that rows are written whole
+            const float sum = l + __shfl_xor(l, 32);
+            const float f = a.splits != 1 ? 1.0f : sum == 0 ? 0.0f : 1.0f / sum;
+            if (a.splits != 1 && half == 0 && tile * kWide + col < cols) {
+                const uint32_t cc = tile * kWide + col, row = over(cc, a.group);
+                float* ml = a.part + static_cast<size_t>(a.b.rows) * a.heads * a.splits * HD +
+                            ((static_cast<size_t>(sr.begin + row) * a.heads + h * a.group.d + (cc - row * a.group.d)) * a.splits + split) * 2;
+                ml[0] = m;
+                ml[1] = sum;
+            }
+#pragma unroll 1
+            for (int c0 = 0; c0 < kWide; c0 += 16) {
+                if (col / 16 == c0 / 16) {
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                const float sum = l[c] + __shfl_xor(l[c], 32);
-                const float f = a.splits != 1 ? 1.0f : sum == 0 ? 0.0f : 1.0f / sum;
+                    for (int b = 0; b < NB; ++b) {
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        float4v y;
-                        for (int r = 0; r < 4; ++r) y[r] = sum == 0 ? 0.0f : acc[c][b][4 * x + r] * f;
-                        *reinterpret_cast<float4v*>(&lds.out[wave][col][32 * b + 8 * x + 4 * half]) = y;
+                        for (int x = 0; x < 4; ++x) {
+                            float4v y;
+                            for (int r = 0; r < 4; ++r) y[r] = sum == 0 ? 0.0f : acc[b][4 * x + r] * f;
+                            *reinterpret_cast<float4v*>(&lds.out[wave][col % 16][32 * b + 8 * x + 4 * half]) = y;
+                        }
                     }
-                }
-                const uint32_t cc = tile[c] * kWide + col;
-                if (a.splits != 1 && half == 0 && cc < cols) {
-                    const uint32_t row = over(cc, a.group);
-                    float* ml = a.part + static_cast<size_t>(a.b.rows) * a.heads * a.splits * HD +
-                                ((static_cast<size_t>(sr.begin + row) * a.heads + h * a.group.d + (cc - row * a.group.d)) * a.splits + split) * 2;
-                    ml[0] = m[c];
-                    ml[1] = sum;
                 }
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-                for (int n = lane; n < kWide * (HD / 8); n += 64) {
+                for (int n = lane; n < 16 * (HD / 8); n += 64) {
                     const int r = n / (HD / 8), d = n % (HD / 8) * 8;
-                    const uint32_t oc = tile[c] * kWide + r;
+                    const uint32_t oc = tile * kWide + c0 + r;
                     if (oc >= cols) continue;
                     const uint32_t row = over(oc, a.group), head = h * a.group.d + (oc - row * a.group.d);
                     const float4v *from = reinterpret_cast<const float4v*>(&lds.out[wave][r][d]), lo = from[0], hi = from[1];
@@ -439,26 +497,37 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1))
     }
 }
 
-template <int NB, int CT>
-hipError_t launch_typed(const PagedAttnArgs& a, dim3 grid, hipStream_t st) {
-    if (a.kv.q4) k_paged_prompt<NB, CT, true><<<grid, dim3(64 * kWaves), 0, st>>>(a);
-    else k_paged_prompt<NB, CT, false><<<grid, dim3(64 * kWaves), 0, st>>>(a);
+template <int NB>
+hipError_t launch_typed(const PagedAttnArgs& a, bool exact, dim3 grid, hipStream_t st) {
+    const dim3 threads(64 * kWaves);
+    if (!exact) {
+        if (a.kv.q4) k_paged_prompt<NB, true, false><<<grid, threads, 0, st>>>(a);
+        else k_paged_prompt<NB, false, false><<<grid, threads, 0, st>>>(a);
+    } else if constexpr (NB <= 4) {
+        if (a.kv.q4) k_paged_prompt<NB, true, true><<<grid, threads, 0, st>>>(a);
+        else k_paged_prompt<NB, false, true><<<grid, threads, 0, st>>>(a);
+    } else {
+        return hipErrorInvalidValue;
+    }
     return hipGetLastError();
 }
 
 }  // namespace
 
-uint32_t prompt_columns(uint32_t head_dim) { return head_dim <= 128 ? 2 * kWide * kWaves : kWide * kWaves; }
+uint32_t prompt_columns() { return kWide * kWaves; }
 
-hipError_t launch_paged_prompt(const PagedAttnArgs& a, uint32_t max_rows, hipStream_t st) {
-    const uint32_t wide = prompt_columns(a.kv.head_dim);
+// 32-bit results take twice the registers and, of 4-bit caches, twice the LDS: heads of up to 128 values.
+bool prompt_fits(uint32_t head_dim, bool exact) { return head_dim <= (exact ? 128 : 256); }
+
+hipError_t launch_paged_prompt(const PagedAttnArgs& a, bool exact, uint32_t max_rows, hipStream_t st) {
+    const uint32_t wide = prompt_columns();
     const uint64_t cols = static_cast<uint64_t>(max_rows) * a.group.d, sets = std::min<uint64_t>((cols + wide - 1) / wide, 65535 / a.splits);
     const dim3 grid(a.kv.kv_heads, static_cast<uint32_t>(sets * a.splits), std::min<uint32_t>(a.b.seqs, 65535));
     switch (a.kv.head_dim / 32) {
-        case 2: return launch_typed<2, 2>(a, grid, st);
-        case 3: return launch_typed<3, 2>(a, grid, st);
-        case 4: return launch_typed<4, 2>(a, grid, st);
-        case 8: return launch_typed<8, 1>(a, grid, st);
+        case 2: return launch_typed<2>(a, exact, grid, st);
+        case 3: return launch_typed<3>(a, exact, grid, st);
+        case 4: return launch_typed<4>(a, exact, grid, st);
+        case 8: return launch_typed<8>(a, exact, grid, st);
     }
     return hipErrorInvalidValue;
 }
