@@ -16,6 +16,15 @@ __device__ inline char* row_ptr(const HeadRows& x, int64_t row, int64_t head) {
     return static_cast<char*>(x.data) + (row * x.row + head * x.head) * (x.type == kTypeF32 ? 4 : 2);
 }
 
+// page_of for a position that is the same for the whole wave and not before 0, of a table that is not empty:
+// a scalar load and no branch.
+__device__ inline int32_t wave_page(const PagedKv& kv, const PagedBatch& b, uint32_t s, int32_t pos) {
+    const uint32_t e = static_cast<uint32_t>(pos) >> kv.page_shift, in = e < b.page_stride ? e : b.page_stride - 1;
+    typedef const __attribute__((address_space(4))) int32_t* Table;
+    const int32_t p = ((Table)(uintptr_t)b.page_table)[static_cast<size_t>(s) * b.page_stride + in];
+    return e < b.page_stride && static_cast<uint32_t>(p) < kv.pages ? p : -1;
+}
+
 __device__ inline float from_bf16(uint32_t b) { return __builtin_bit_cast(float, b << 16); }
 __device__ inline float from_half(uint32_t h) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h))); }
 __device__ inline uint32_t to_half(float x) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x)); }
@@ -117,13 +126,13 @@ __device__ inline Marks scale_marks(uint32_t w) {  // blocks without a scale are
     return {i * 0x7800, i * 0x7800, w & ~(i * 0xFFFF)};
 }
 
-template <int N>
-struct alignas(N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4) Words {
+template <int N, int ALIGN>
+struct alignas(ALIGN) Words {
     uint32_t w[N];
 };
-template <int N>
+template <int N, int ALIGN = N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4>
 __device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {
-    const Words<N> x = *reinterpret_cast<const Words<N>*>(p);
+    const Words<N, ALIGN> x = *reinterpret_cast<const Words<N, ALIGN>*>(p);
     for (int k = 0; k < N; ++k) w[k] = x.w[k];
 }
 

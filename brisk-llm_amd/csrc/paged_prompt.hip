@@ -14,99 +14,82 @@ namespace bh {
 namespace {
 
 constexpr int kWaves = 8;
-constexpr int kBlock = 64;  // positions in LDS at a time: four tiles, of each of which one wave unpacks the keys, one the values
+constexpr int kBlock = 64;  // positions of a wave's step
 constexpr int kVector = 0x2, kMfma = 0x8;  // instructions' classes, for their order
 constexpr int kWide = 32;   // columns of a wave: (row, head) pairs of a key/value head
 
-// What a thread holds of its wave's keys or values until they go to LDS.
+// What a thread holds of its wave's half of a tile, blocks b0 .. b0 + HB - 1 of every position, until it goes to LDS.
 template <int NB, bool Q4>
 struct RawTile {
-    static constexpr int GS = NB < 4 ? NB : 4, NG = NB / GS;
-    uint32_t w[NG][Q4 ? 1 : 4][GS], s[NG][Q4 ? 2 * GS : 1];
+    static constexpr int GS = NB < 4 ? NB : 4, HB = (NB + 1) / 2, ALIGN = NB % 4 == 0 ? HB * 4 : 4;
+    uint32_t k[HB][Q4 ? 1 : 4], ks[Q4 ? HB : 1], v[Q4 ? 1 : 4][HB], vs[Q4 ? 2 * HB : 1];
 
-    __device__ inline void load_keys(const uint8_t* tile, int lane) {
+    // (of three blocks both halves take the middle one)
+    static __device__ inline int first(int part) { return part ? NB - HB : 0; }
+
+    __device__ inline void load(const uint8_t* tile, int b0, int lane) {
+        const uint32_t at = ((b0 / GS * 64 + lane) * GS + b0 % GS) * 4;
+        if constexpr (Q4) {
+            uint32_t x[HB];
+            load_words<HB, ALIGN>(tile + at, x);
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            if constexpr (Q4) {
-                load_words<GS>(tile + (n * 64 + lane) * GS * 4, w[n][0]);
-#pragma unroll
-                for (int e = 0; e < GS; ++e)  // the lane's position's scale, twice
-                    s[n][e] = *reinterpret_cast<const uint16_t*>(tile + scale_offset(NB, false, lane % 16, n * GS + e)) * 0x10001u;
-            } else {
-#pragma unroll
-                for (int e = 0; e < GS; ++e) {
-                    const word4v x = *reinterpret_cast<const word4v*>(tile + ((n * GS + e) * 64 + lane) * 16);
-                    for (int j = 0; j < 4; ++j) w[n][j][e] = x[j];
-                }
+            for (int j = 0; j < HB; ++j) {
+                k[j][0] = x[j];
+                ks[j] = *reinterpret_cast<const uint16_t*>(tile + scale_offset(NB, false, lane % 16, b0 + j)) * 0x10001u;  // the lane's position's, twice
             }
-        }
-    }
-    __device__ inline void load_values(const uint8_t* tile, int lane) {
-        const uint8_t* at = tile + tile_values_at(Q4, NB);
+            load_words<HB, ALIGN>(tile + tile_values_at(true, NB) + at, v[0]);
+            load_words<2 * HB, 8>(tile + tile_value_scales_at(NB) + (lane / 16 * NB + b0) * 8, vs);
+        } else {
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            if constexpr (Q4) {
-                load_words<GS>(at + (n * 64 + lane) * GS * 4, w[n][0]);
-                load_words<2 * GS>(tile + tile_value_scales_at(NB) + (lane / 16 * NB + n * GS) * 8, s[n]);
-            } else {
+            for (int j = 0; j < HB; ++j) load_words<4>(tile + ((b0 + j) * 64 + lane) * 16, k[j]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) load_words<GS>(at + ((r * NG + n) * 64 + lane) * GS * 4, w[n][r]);
-            }
+            for (int r = 0; r < 4; ++r) load_words<HB, ALIGN>(tile + tile_values_at(false, NB) + r * NB * 256 + at, v[r]);
         }
     }
     // The values of positions 4 g + r whose bit r of `keep` is not set become zeros.
     __device__ inline void keep_values(uint32_t keep) {
+        if constexpr (Q4) {
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            if constexpr (Q4) {
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t b = keep >> (2 * j), mask = (b & 1 ? 0xFFFF : 0) | (b & 2 ? 0xFFFF0000 : 0);
+                for (int e = 0; e < HB; ++e) vs[2 * e + j] &= mask;
+            }
+        } else {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t b = keep >> (2 * j), mask = (b & 1 ? 0xFFFF : 0) | (b & 2 ? 0xFFFF0000 : 0);
-                    for (int e = 0; e < GS; ++e) s[n][2 * e + j] &= mask;
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t mask = keep >> r & 1 ? 0xFFFFFFFF : 0;
-                    for (int e = 0; e < GS; ++e) w[n][r][e] &= mask;
-                }
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t mask = keep >> r & 1 ? 0xFFFFFFFF : 0;
+                for (int e = 0; e < HB; ++e) v[r][e] &= mask;
             }
         }
     }
     // Whether an infinity or NaN is among the values; and zeros in their place.
     __device__ inline bool any_ill() const {
         uint32_t found = 0;
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            if constexpr (Q4) {
-                for (int e = 0; e < 2 * GS; ++e) found |= ill<true>(s[n][e]);
-            } else {
-                for (int r = 0; r < 4; ++r)
-                    for (int e = 0; e < GS; ++e) found |= ill<false>(w[n][r][e]);
-            }
+        if constexpr (Q4) {
+            for (int e = 0; e < 2 * HB; ++e) found |= ill<true>(vs[e]);
+        } else {
+            for (int r = 0; r < 4; ++r)
+                for (int e = 0; e < HB; ++e) found |= ill<false>(v[r][e]);
         }
         return __any((found & kIll) != 0);
     }
     __device__ inline void drop_ill() {
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            if constexpr (Q4) {
-                for (int e = 0; e < 2 * GS; ++e) s[n][e] = scale_marks(s[n][e]).rest;
-            } else {
-                for (int r = 0; r < 4; ++r)
-                    for (int e = 0; e < GS; ++e) w[n][r][e] = marks(w[n][r][e]).rest;
-            }
+        if constexpr (Q4) {
+            for (int e = 0; e < 2 * HB; ++e) vs[e] = scale_marks(vs[e]).rest;
+        } else {
+            for (int r = 0; r < 4; ++r)
+                for (int e = 0; e < HB; ++e) v[r][e] = marks(v[r][e]).rest;
         }
     }
 };
 
-// Operands [32 positions][16 dimensions] and [32 dimensions][16 positions], 64 lanes x 16 bytes each, in one plane or,
-// for 4-bit values with 32-bit results, in two that add up to them.
-template <int NB, int PLANES>
+// STEPS x 64 positions as operands [32 positions][16 dimensions] and [32 dimensions][16 positions], 64 lanes x 16 bytes
+// each, in one plane or, for 4-bit values with 32-bit results, in two that add up to them.
+template <int NB, int PLANES, int STEPS>
 struct BlockLds {
-    word4v k[PLANES][kBlock / 32][2 * NB][64];
-    word4v v[PLANES][NB][kBlock / 16][64];
-    uint8_t there[kBlock / 16], poison[kBlock / 16];  // whether a tile is there, and holds values that are not finite (here they are zeros)
+    word4v k[PLANES][STEPS * 2][2 * NB][64];
+    word4v v[PLANES][NB][STEPS * 4][64];
+    uint8_t there[kWaves], poison[kWaves];  // whether a wave's half tile is there, and holds values that are not finite (here they are zeros)
 };
 
 // A code times its scale, in one half (rounded: 2^-11 of the value at most, as the probabilities are), or in two (exact).
@@ -117,41 +100,29 @@ __device__ inline void scaled(half2v code, uint32_t scale, uint32_t (&out)[PLANE
     if constexpr (PLANES == 2) out[1] = bits(__builtin_elementwise_fma(code, d, -x));
 }
 
-template <int NB, bool Q4, int PLANES>
-__device__ inline void unpack_keys(const RawTile<NB, Q4>& raw, BlockLds<NB, PLANES>& out, int x, int lane) {
-    constexpr int GS = NB < 4 ? NB : 4;
+template <int NB, bool Q4, int PLANES, int STEPS>
+__device__ inline void unpack(const RawTile<NB, Q4>& raw, BlockLds<NB, PLANES, STEPS>& out, int x, int b0, int lane) {
     const int i = lane % 16, g = lane / 16;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int n = b / GS, e = b % GS;
-        uint32_t y[4][PLANES];
+    for (int j = 0; j < RawTile<NB, Q4>::HB; ++j) {
+        uint32_t key[4][PLANES];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (Q4) scaled<PLANES>(codes(raw.w[n][0][e] >> (j / 2 * 8), j % 2), raw.s[n][e], y[j]);
-            else y[j][0] = raw.w[n][j][e];
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (Q4) scaled<PLANES>(codes(raw.k[j][0] >> (e / 2 * 8), e % 2), raw.ks[j], key[e]);
+            else key[e][0] = raw.k[j][e];
         }
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) out.k[p][x / 2][2 * b + g / 2][g % 2 * 32 + x % 2 * 16 + i] = word4v{y[0][p], y[1][p], y[2][p], y[3][p]};
-    }
-}
-
-template <int NB, bool Q4, int PLANES>
-__device__ inline void unpack_values(const RawTile<NB, Q4>& raw, BlockLds<NB, PLANES>& out, int x, int lane) {
-    constexpr int GS = NB < 4 ? NB : 4;
-    const int i = lane % 16, g = lane / 16;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int n = b / GS, e = b % GS;
+        for (int p = 0; p < PLANES; ++p) out.k[p][x / 2][2 * (b0 + j) + g / 2][g % 2 * 32 + x % 2 * 16 + i] = word4v{key[0][p], key[1][p], key[2][p], key[3][p]};
 #pragma unroll
         for (int c2 = 0; c2 < 2; ++c2) {
-            uint32_t y[2][PLANES];
+            uint32_t val[2][PLANES];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                if constexpr (Q4) scaled<PLANES>(codes(raw.w[n][0][e] >> (j * 8), c2), raw.s[n][2 * e + j], y[j]);
-                else y[j][0] = __builtin_amdgcn_perm(raw.w[n][2 * j + 1][e], raw.w[n][2 * j][e], c2 ? 0x07060302 : 0x05040100);
+            for (int e = 0; e < 2; ++e) {
+                if constexpr (Q4) scaled<PLANES>(codes(raw.v[0][j] >> (e * 8), c2), raw.vs[2 * j + e], val[e]);
+                else val[e][0] = __builtin_amdgcn_perm(raw.v[2 * e + 1][j], raw.v[2 * e][j], c2 ? 0x07060302 : 0x05040100);
             }
 #pragma unroll
-            for (int p = 0; p < PLANES; ++p) reinterpret_cast<word2v*>(&out.v[p][b][x][g % 2 * 32 + 2 * i + c2])[g / 2] = word2v{y[0][p], y[1][p]};
+            for (int p = 0; p < PLANES; ++p) reinterpret_cast<word2v*>(&out.v[p][b0 + j][x][g % 2 * 32 + 2 * i + c2])[g / 2] = word2v{val[0][p], val[1][p]};
         }
     }
 }
@@ -162,8 +133,12 @@ __device__ inline void unpack_values(const RawTile<NB, Q4>& raw, BlockLds<NB, PL
 template <int NB, bool Q4, bool EXACT>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_paged_prompt(PagedAttnArgs a) {
     constexpr int HD = 32 * NB, PLANES = Q4 && EXACT ? 2 : 1, PARTS = EXACT ? 2 : 1;
+    // Two blocks in LDS, one multiplied while the other is filled: of 128 positions, a tile for each wave, where they fit
+    // (two 64-KB blocks), otherwise of 64, half a tile for each.
+    constexpr int STEPS = NB * PLANES <= 4 ? 2 : 1, BLOCK = STEPS * kBlock;
+    typedef BlockLds<NB, PLANES, STEPS> Block;
     __shared__ union {
-        BlockLds<NB, PLANES> block[2];
+        Block block[2];
         struct {
             _Float16 part[PARTS][kWaves][16][HD + 8];  // (half of a wave's columns at a time)
             float scale[kWaves][16];
@@ -196,44 +171,60 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             int32_t pos_lo = 0, pos_hi = 0, t_lo = 0, t_hi = 0;
             if (tile < tiles) range(tile, pos_lo, pos_hi, t_lo, t_hi);
             const int32_t pos = tile * kWide + col < cols ? sr.first + static_cast<int32_t>(over(tile * kWide + col, a.group)) : pos_lo;
-            int32_t wg_lo, wg_plo, wg_phi, wg_hi, x0, x1, x2;  // the workgroup's, from its first tile's to its last one's
-            range(front, wg_plo, x0, wg_lo, x1);
-            range(window == 0 ? tiles - 1 - front : back_last, x0, wg_phi, x2, wg_hi);
-            const int32_t blk_lo = wg_lo / kBlock, blocks = wg_hi > wg_lo ? (wg_hi + kBlock - 1) / kBlock - blk_lo : 0;
+            int32_t wg_lo, wg_plo, wg_phi, wg_hi, y0, y1, y2;  // the workgroup's, from its first tile's to its last one's
+            range(front, wg_plo, y0, wg_lo, y1);
+            range(window == 0 ? tiles - 1 - front : back_last, y0, wg_phi, y2, wg_hi);
+            const int32_t blk_lo = wg_lo / BLOCK, blocks = wg_hi > wg_lo ? (wg_hi + BLOCK - 1) / BLOCK - blk_lo : 0;
             const int32_t per = (blocks + static_cast<int32_t>(a.splits) - 1) / static_cast<int32_t>(a.splits);
             const int32_t blk_begin = blk_lo + static_cast<int32_t>(std::min<int64_t>(blocks, static_cast<int64_t>(per) * split));
             const int32_t blk_end = blk_lo + static_cast<int32_t>(std::min<int64_t>(blocks, static_cast<int64_t>(per) * (split + 1)));
 
-            RawTile<NB, Q4> raw;
-            bool there = false;
-            const bool keys = wave < 4;
-            const auto fetch = [&](int32_t blk) {
-                const int32_t t = blk * kBlock + 16 * (wave & 3), page = page_of(a.kv, a.b, s, t);
-                there = page >= 0;
-                const uint8_t* from = a.kv.data + tile_at(a.kv, there ? page : 0, h, t);
-                if (keys) raw.load_keys(from, lane);
-                else raw.load_values(from, lane);
+            RawTile<NB, Q4> raw[STEPS];
+            bool there = false, poison = false;
+            const int x = STEPS == 2 ? wave : wave & 3;
+            const auto part = [&](int step) { return RawTile<NB, Q4>::first(STEPS == 2 ? step : wave >> 2); };
+            const auto page_at = [&](int32_t blk) { return wave_page(a.kv, a.b, s, blk * BLOCK + 16 * x); };
+            int32_t page = -1, page_next = -1;
+            const auto fetch = [&](int32_t blk, int step) {
+                raw[step].load(a.kv.data + tile_at(a.kv, page < 0 ? 0 : page, h, blk * BLOCK + 16 * x), part(step), lane);
             };
-            const auto put = [&](int32_t blk) {
-                BlockLds<NB, PLANES>& out = lds.block[blk & 1];
-                if (keys) {
-                    unpack_keys<NB, Q4, PLANES>(raw, out, wave, lane);
-                    if (lane == 0) out.there[wave] = there;
-                    return;
-                }
-                // some column does not see all of the block: what none sees is left out
-                if (!there || (blk + 1) * kBlock - 1 > wg_plo || (window != 0 && blk * kBlock <= wg_phi - window)) {
-                    const int32_t t = blk * kBlock + 16 * (wave & 3) + 4 * (lane / 16);
+            // some column does not see all of a block: what none sees is left out; and what is not finite
+            const auto check = [&](int32_t blk) {
+                if (!there || (blk + 1) * BLOCK - 1 > wg_plo || (window != 0 && blk * BLOCK <= wg_phi - window)) {
+                    const int32_t t = blk * BLOCK + 16 * x + 4 * (lane / 16);
                     uint32_t keep = 0;
                     for (int r = 0; r < 4; ++r) keep |= there && t + r >= wg_lo && t + r <= wg_phi ? 1u << r : 0;
-                    raw.keep_values(keep);
+#pragma unroll
+                    for (int step = 0; step < STEPS; ++step) raw[step].keep_values(keep);
                 }
-                const bool poison = raw.any_ill();
-                if (__builtin_expect(poison, 0)) raw.drop_ill();
-                unpack_values<NB, Q4, PLANES>(raw, out, wave & 3, lane);
-                if (lane == 0) out.poison[wave & 3] = poison;
+                poison = raw[0].any_ill();
+                if constexpr (STEPS == 2) poison |= raw[1].any_ill();
+                if (__builtin_expect(poison, 0)) {
+#pragma unroll
+                    for (int step = 0; step < STEPS; ++step) raw[step].drop_ill();
+                }
             };
-            if (blk_begin < blk_end) fetch(blk_begin);
+            const auto put = [&](int32_t blk, int step) {
+                Block& out = lds.block[blk & 1];
+                unpack<NB, Q4, PLANES, STEPS>(raw[step], out, x, part(step), lane);
+                out.there[wave] = there;  // (every lane the same: a branch would end the block of instructions that is scheduled)
+                out.poison[wave] = poison;
+            };
+            // A part of the next block goes to LDS; then the same part of the block after it is fetched, of a page whose number
+            // was read a block before.
+            const auto next = [&](int32_t blk, int step) {
+                if (step == 0) {
+                    page = page_next;
+                    page_next = page_at(blk + 3);
+                }
+                fetch(blk + 2, step);
+            };
+            if (blk_begin < blk_end) {
+                page = page_at(blk_begin);
+                page_next = page_at(blk_begin + 1);
+#pragma unroll
+                for (int step = 0; step < STEPS; ++step) fetch(blk_begin, step);
+            }
 
             // the columns' queries, through the wave's part of LDS: 16 lanes a column, scaled by a power of two where the
             // type has more range than a half, and by the sign of the score's scale
@@ -292,17 +283,20 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[b] = float16v{};
 
-            // a block of 64 positions from t0 on: two products of 32 side by side, since one's steps wait for each other
-            const auto sub = [&](const BlockLds<NB, PLANES>& in, int32_t t0) {
-                const uint32_t there = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t*>(in.there));
-                const uint32_t poison = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const uint32_t*>(in.poison));
+            // A block of 64 positions from t0 on: two products of 32 side by side, since one's steps wait for each other;
+            // the next block is unpacked under them.
+            const auto sub = [&](const Block& in, int32_t blk, int step) {
+                const int32_t t0 = blk * BLOCK + step * kBlock;
+                const uint32_t heres = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(in.there)[step]);
+                const uint32_t* ill_at = reinterpret_cast<const uint32_t*>(in.poison);
+                const uint32_t ills = __builtin_amdgcn_readfirstlane(STEPS == 2 ? ill_at[step] : ill_at[0] | ill_at[1]);
                 float16v sc[2] = {};
                 // The operands of half of the steps are read ahead of the products of the other half; the
                 // barriers keep the compiler from undoing that.
                 const auto read_keys = [&](half8v (&x)[PLANES][2 * NB], int k0) {
 #pragma unroll
                     for (int k = 0; k < 2 * NB; ++k)
-                        for (int e = 0; e < PLANES; ++e) x[e][k] = __builtin_bit_cast(half8v, in.k[e][k % 2][k0 + k / 2][lane]);
+                        for (int e = 0; e < PLANES; ++e) x[e][k] = __builtin_bit_cast(half8v, in.k[e][2 * step + k % 2][k0 + k / 2][lane]);
                 };
                 const auto keys_times = [&](const half8v (&x)[PLANES][2 * NB], int k0) {
 #pragma unroll
@@ -319,27 +313,37 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 __builtin_amdgcn_sched_barrier(0);
                 read_keys(ops[1], NB);
                 __builtin_amdgcn_sched_barrier(0);
+                put(blk + 1, step);
                 keys_times(ops[0], 0);
                 keys_times(ops[1], NB);
+                if constexpr (!EXACT) {
+#pragma unroll
+                    for (int k = 0; k < 4 * NB; ++k) {
+                        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(kVector, 4, 0);
+                    }
+                }
                 __builtin_amdgcn_sched_barrier(0);
+                next(blk, step);
                 // the values' operands likewise, of 32 positions at a time
                 const auto read_values = [&](half8v (&x)[PLANES][2 * NB], int u0) {
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
                         for (int b = 0; b < NB; ++b)
-                            for (int e = 0; e < PLANES; ++e) x[e][u * NB + b] = __builtin_bit_cast(half8v, in.v[e][b][u0 + u][lane]);
+                            for (int e = 0; e < PLANES; ++e) x[e][u * NB + b] = __builtin_bit_cast(half8v, in.v[e][b][4 * step + u0 + u][lane]);
                 };
                 read_values(ops[0], 0);
                 __builtin_amdgcn_sched_barrier(0);
                 // the column sees positions t0 + u with lo < u <= hi, in tiles that are there
                 const int32_t hi = pos - t0, lo = window != 0 ? hi - window : -1;
-                if (there != 0x01010101 || t0 + kBlock - 1 > pos_lo || (window != 0 && t0 <= pos_hi - window)) {
+                if (heres != 0x01010101 || t0 + kBlock - 1 > pos_lo || (window != 0 && t0 <= pos_hi - window)) {
+                    asm volatile("");  // a branch, not 32 selects for every block
 #pragma unroll
                     for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const int32_t u = 32 * tt + 8 * (r / 4) + 4 * half + r % 4;
-                            if (u > hi || u <= lo || (there >> (16 * tt + r / 8 * 8) & 1) == 0) sc[tt][r] = -__builtin_inff();
+                            if (u > hi || u <= lo || (heres >> (16 * tt + r / 8 * 8) & 1) == 0) sc[tt][r] = -__builtin_inff();
                         }
                     }
                 }
@@ -409,11 +413,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 __builtin_amdgcn_sched_barrier(0);
                 values_times(ops[1], 2);
                 l += sums[0] + sums[1];
-                if (__builtin_expect(poison != 0, 0)) {
+                if (__builtin_expect(ills != 0, 0)) {
                     // the values that are not finite, from the tiles themselves
 #pragma unroll 1
                     for (int u = 0; u < 4; ++u) {
-                        const int32_t t = t0 + 16 * u, page = page_of(a.kv, a.b, s, t);
+                        const int32_t t = t0 + 16 * u, page = wave_page(a.kv, a.b, s, t);
                         const uint8_t* from = a.kv.data + tile_at(a.kv, page < 0 ? 0 : page, h, t);
                         half8v sees;
 #pragma unroll
@@ -441,14 +445,29 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 }
             };
 
-            if (blk_begin < blk_end) put(blk_begin);
+            if (blk_begin < blk_end) {
+                there = page >= 0;
+                check(blk_begin);
+#pragma unroll
+                for (int step = 0; step < STEPS; ++step) {
+                    put(blk_begin, step);
+                    next(blk_begin - 1, step);
+                }
+            }
             __syncthreads();
             for (int32_t blk = blk_begin; blk < blk_end; ++blk) {
-                if (blk + 1 < blk_end) fetch(blk + 1);
-                const BlockLds<NB, PLANES>& in = lds.block[blk & 1];
-                const int32_t t0 = blk * kBlock;
-                if (t0 < t_hi && t0 + kBlock > t_lo) sub(in, t0);
-                if (blk + 1 < blk_end) put(blk + 1);
+                there = page >= 0;
+                check(blk + 1);
+#pragma unroll
+                for (int step = 0; step < STEPS; ++step) {
+                    const int32_t t0 = blk * BLOCK + step * kBlock;
+                    if (t0 < t_hi && t0 + kBlock > t_lo) {
+                        sub(lds.block[blk & 1], blk, step);
+                    } else {
+                        put(blk + 1, step);
+                        next(blk, step);
+                    }
+                }
                 __syncthreads();
             }
 
