@@ -154,6 +154,11 @@ bh::PagedBatch paged_batch(const brisk_hip_batch* b, bool data) {
     return {b->row_start, b->lengths, b->page_table, b->seqs, b->rows, b->page_stride, b->max_rows, b->max_length};
 }
 
+bh::Divisor cache_pairs(const bh::PagedKv& kv, const bh::PagedBatch& b) {
+    if ((static_cast<uint64_t>(b.rows) + 32) * kv.kv_heads * 2 > 0x7FFFFFFFu) bad("too many rows and heads");
+    return bh::divisor(2 * kv.kv_heads);
+}
+
 uint32_t head_group(uint32_t heads, const bh::PagedKv& kv) {
     if (heads == 0 || heads > 65536 || heads % kv.kv_heads != 0) bad("the query heads must be a multiple of the key/value heads");
     return heads / kv.kv_heads;
@@ -387,6 +392,8 @@ int brisk_hip_qk_norm_rope(const brisk_hip_heads* q, const brisk_hip_heads* k, s
         a.heads[0] = heads;
         a.heads[1] = kv_heads;
         a.head_dim = head_dim;
+        a.all = bh::divisor(heads + (k != nullptr ? kv_heads : 0));
+        if (static_cast<uint64_t>(n) * a.all.d > 0x7FFFFFFFu) bad("too many rows and heads");
         a.n = n;
         a.eps = eps;
         a.positions = positions;
@@ -405,6 +412,7 @@ int brisk_hip_kv_append(const brisk_hip_kv* kv, const brisk_hip_batch* batch, co
         if (a.b.rows == 0 || a.b.seqs == 0) return;
         a.k = head_rows(k, "keys");
         a.v = head_rows(v, "values");
+        a.pairs = cache_pairs(a.kv, a.b);
         a.w = k_norm;
         a.eps = eps;
         hip_check(bh::launch_kv_append(a, static_cast<hipStream_t>(stream)), "kv_append");
@@ -421,6 +429,7 @@ int brisk_hip_kv_read(const brisk_hip_kv* kv, const brisk_hip_batch* batch, cons
         if (k != nullptr) a.k = written_rows(k, "keys", a.b.rows, a.kv.kv_heads, a.kv.head_dim);
         if (v != nullptr) a.v = written_rows(v, "values", a.b.rows, a.kv.kv_heads, a.kv.head_dim);
         if (k == nullptr && v == nullptr) return;
+        a.pairs = cache_pairs(a.kv, a.b);
         hip_check(bh::launch_kv_read(a, static_cast<hipStream_t>(stream)), "kv_read");
     });
 }

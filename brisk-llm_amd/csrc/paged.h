@@ -140,6 +140,7 @@ struct NormRopeArgs {
     HeadRows x[2], y[2];    // queries and keys; x[1].data null: no keys
     const float* w[2];      // norm weights, or null
     uint32_t heads[2], head_dim;
+    Divisor all;  // heads a row, of both
     size_t n;
     float eps;
     RopeTable rope;
@@ -151,6 +152,7 @@ struct AppendArgs {
     PagedKv kv;
     PagedBatch b;
     HeadRows k, v;
+    Divisor pairs;   // 2 x key/value heads
     const float* w;  // the keys' norm weights, or null
     float eps;
     RopeTable rope;
@@ -161,6 +163,7 @@ struct ReadArgs {
     PagedKv kv;
     PagedBatch b;
     HeadRows k, v;  // data null: not wanted
+    Divisor pairs;  // 2 x key/value heads
 };
 hipError_t launch_kv_read(const ReadArgs& a, hipStream_t st);
 

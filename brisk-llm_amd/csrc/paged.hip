@@ -94,13 +94,13 @@ __device__ inline void turned(const void* head, int type, bool vec, int d, int h
 // One group of lanes a head.  A head's lanes read all they need before they write, so y may be x.
 __global__ __launch_bounds__(kThreads) void k_norm_rope(NormRopeArgs a, int lanes, int vec) {
     const int lane = static_cast<int>(threadIdx.x) % lanes, d = lane * 8;
-    const size_t per = kThreads / lanes, all = a.heads[0] + (a.x[1].data != nullptr ? a.heads[1] : 0), total = a.n * all;
+    const uint32_t per = kThreads / lanes, total = static_cast<uint32_t>(a.n) * a.all.d;
     // the shuffles of a group want its whole wave in the loop: the bound is the block's first head
-    for (size_t base = blockIdx.x * per; base < total; base += static_cast<size_t>(gridDim.x) * per) {
-        const size_t u = base + threadIdx.x / lanes;
+    for (uint32_t base = blockIdx.x * per; base < total; base += gridDim.x * per) {
+        const uint32_t u = base + threadIdx.x / lanes;
         const bool in = u < total;
-        const size_t row = in ? u / all : 0;
-        uint32_t h = in ? static_cast<uint32_t>(u % all) : 0;
+        const uint32_t row = in ? over(u, a.all) : 0;
+        uint32_t h = in ? u - row * a.all.d : 0;
         const int t = h >= a.heads[0] ? 1 : 0;
         if (t) h -= a.heads[0];
         const float* cs = nullptr;
@@ -171,17 +171,18 @@ __global__ __launch_bounds__(kThreads) void k_kv_append(AppendArgs a, int lanes,
     const int lane = static_cast<int>(threadIdx.x) % lanes, d = lane * 8, hd = static_cast<int>(a.kv.head_dim);
     const uint32_t nb = a.kv.head_dim / 32;
     const bool q4 = a.kv.q4 != 0, live = d < hd;
-    const int64_t per = kThreads / lanes, heads = a.kv.kv_heads;
+    const uint32_t per = kThreads / lanes, heads = a.kv.kv_heads;
     for (uint32_t s = blockIdx.y; s < a.b.seqs; s += gridDim.y) {
         const SeqRows sr = seq_rows(a.b, s);
-        const int64_t total = static_cast<int64_t>(sr.end - sr.begin) * heads * 2;
-        for (int64_t base = blockIdx.x * per; base < total; base += static_cast<int64_t>(gridDim.x) * per) {
-            const int64_t u = base + threadIdx.x / lanes;
+        const uint32_t total = (sr.end - sr.begin) * heads * 2;
+        for (uint32_t base = blockIdx.x * per; base < total; base += gridDim.x * per) {
+            const uint32_t u = base + threadIdx.x / lanes;
             const bool in = u < total;
-            const int64_t row = sr.begin + (in ? u / (2 * heads) : 0);
-            const uint32_t h = in ? static_cast<uint32_t>(u % heads) : 0;
-            const bool value = in && u % (2 * heads) >= heads;
-            const int32_t pos = sr.first + static_cast<int32_t>(row - sr.begin);
+            const uint32_t n = in ? over(u, a.pairs) : 0, row = sr.begin + n;
+            uint32_t h = in ? u - n * a.pairs.d : 0;
+            const bool value = h >= heads;
+            if (value) h -= heads;
+            const int32_t pos = sr.first + static_cast<int32_t>(n);
             const int32_t page = page_of(a.kv, a.b, s, pos);
             bool keep = !in || page < 0;
             const float* cs = nullptr;
@@ -222,29 +223,296 @@ __global__ __launch_bounds__(kThreads) void k_kv_append(AppendArgs a, int lanes,
     }
 }
 
-// One group of lanes a row's head of keys, then of values.
-__global__ __launch_bounds__(kThreads) void k_kv_read(ReadArgs a, int lanes, int vec) {
-    const int lane = static_cast<int>(threadIdx.x) % lanes, d = lane * 8;
-    const uint32_t nb = a.kv.head_dim / 32;
-    if (d >= static_cast<int>(a.kv.head_dim)) return;
-    const int64_t per = kThreads / lanes, heads = a.kv.kv_heads;
+// The larger of a value and those of the lanes 16, 32 and 48 away, and the smaller.
+template <bool MAX>
+__device__ inline uint32_t across16(uint32_t x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = MAX ? max(a[0], a[1]) : min(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return MAX ? max(b[0], b[1]) : min(b[0], b[1]);
+}
+
+// Codes of eight values of a block of 32 held by the lanes 16 apart, and the block's scale: as quantise8's,
+// whose comments hold.  Magnitudes are compared as their bits, in which NaN is largest.
+__device__ inline void quantise8_tile(const float (&y)[8], int g, uint32_t (&code)[8], uint16_t& scale) {
+    uint32_t top = 0;
+    for (int j = 0; j < 8; ++j) top = max(top, __builtin_bit_cast(uint32_t, y[j]) & 0x7FFFFFFF);
+    top = across16<true>(top);
+    uint32_t at = 1024;  // the first of them, and its sign
+    for (int j = 7; j >= 0; --j) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, y[j]);
+        if ((b & 0x7FFFFFFF) == top) at = (8 * g + j) * 2 + (b >> 31);
+    }
+    at = across16<false>(at);
+    const float size = __builtin_bit_cast(float, top);
+    const _Float16 ah = static_cast<_Float16>(size * 0.125f);
+    const float a = static_cast<float>(ah);
+    const bool up = at & 1;  // a negative top: a positive scale
+    if (!(a <= kMaxScale)) {
+        scale = 0x7e00;
+        for (int j = 0; j < 8; ++j) code[j] = 8;
+        return;
+    }
+    scale = static_cast<uint16_t>(__builtin_bit_cast(uint16_t, ah) | (up ? 0 : 0x8000));
+    const float inv = a > 0 ? __builtin_amdgcn_rcpf(a) : 0.0f;
+    for (int j = 0; j < 8; ++j) {
+        const float x = up ? y[j] : -y[j];
+        float n = __builtin_floorf(__builtin_fmaf(x, inv, 8.5f));
+        n = __builtin_fminf(__builtin_fmaxf(n, 0.0f), 15.0f);
+        n += x >= (n - 7.5f) * a ? 1.0f : x < (n - 8.5f) * a ? -1.0f : 0.0f;
+        code[j] = a > 0 ? static_cast<uint32_t>(__builtin_fminf(__builtin_fmaxf(n, 0.0f), 15.0f)) : 8;
+    }
+}
+
+// A 4 x 4 transposition of bytes in each four lanes: lane j's byte q, of position j, goes to lane q; a
+// word's positions in the order 0, 2, 1, 3.
+__device__ inline uint32_t transposed(uint32_t w, int lane) {
+    const uint32_t a = __builtin_amdgcn_update_dpp(0, w, 0xB1, 0xF, 0xF, true);  // lanes 1, 0, 3, 2
+    w = __builtin_amdgcn_perm(a, w, lane & 1 ? 0x03070105 : 0x06020400);
+    const uint32_t b = __builtin_amdgcn_update_dpp(0, w, 0x4E, 0xF, 0xF, true);  // lanes 2, 3, 0, 1
+    return __builtin_amdgcn_perm(b, w, lane & 2 ? 0x03070206 : 0x05010400);
+}
+
+// One wave a tile's keys or values: lane 16 g + i has dimensions 32 b + 8 g + 0..7 of position i, for each block b, which is
+// how the tile holds keys.  A rotation's pairs lie in one lane (adjacent, or half the rotated dimensions,
+// whole blocks, apart); norms and quantisation cross four lanes, 4-bit values' bytes four others.
+// Bound by memory in long prompts; rows of single tokens use one lane in 16, and cost a launch.
+template <int NB, bool Q4>
+__global__ __launch_bounds__(kThreads) void k_kv_append_tiles(AppendArgs a) {
+    constexpr int GS = NB < 4 ? NB : 4, NG = NB / GS, HD = 32 * NB;
+    const int lane = static_cast<int>(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = lane % 16, g = lane / 16;
     for (uint32_t s = blockIdx.y; s < a.b.seqs; s += gridDim.y) {
         const SeqRows sr = seq_rows(a.b, s);
-        const int64_t total = static_cast<int64_t>(sr.end - sr.begin) * heads * 2;
-        for (int64_t u = blockIdx.x * per + threadIdx.x / lanes; u < total; u += static_cast<int64_t>(gridDim.x) * per) {
-            const int64_t row = sr.begin + u / (2 * heads);
-            const uint32_t h = static_cast<uint32_t>(u % heads);
-            const bool value = u % (2 * heads) >= heads;
-            const HeadRows& y = value ? a.v : a.k;
-            const int32_t pos = sr.first + static_cast<int32_t>(row - sr.begin), page = page_of(a.kv, a.b, s, pos);
-            if (y.data == nullptr || page < 0) continue;
-            const uint8_t* tile = a.kv.data + tile_at(a.kv, page, h, pos);
-            const uint32_t token = static_cast<uint32_t>(pos) % kTileTokens;
-            float out[8];
-            read8(tile, a.kv.q4 != 0, nb, value, token, d, out);
-            store8(row_ptr(y, row, h), y.type, vec & (value ? 2 : 1), d, out);
+        if (sr.end <= sr.begin) continue;
+        const int32_t last = sr.first + (sr.end - sr.begin) - 1, t_lo = sr.first < 0 ? 0 : sr.first / 16, t_hi = last < 0 ? 0 : last / 16 + 1;
+        const uint32_t total = (t_hi - t_lo) * a.pairs.d;
+        for (uint32_t u = blockIdx.x * 4 + wave; u < total; u += gridDim.x * 4) {
+            const uint32_t n = over(u, a.pairs), rest = u - n * a.pairs.d;
+            const bool value = rest >= a.kv.kv_heads;
+            const uint32_t h = value ? rest - a.kv.kv_heads : rest;
+            const int32_t t0 = (t_lo + static_cast<int32_t>(n)) * 16, page = page_of(a.kv, a.b, s, t0), pos = t0 + i;
+            if (page < 0) continue;
+            const int32_t row = sr.begin + (pos - sr.first);
+            const bool live = row >= sr.begin && row < sr.end && (a.rope.table == nullptr || static_cast<uint32_t>(pos) < a.rope.positions);
+            const bool full = __all(live);
+            if (!__any(live)) continue;
+            uint8_t* tile = a.kv.data + tile_at(a.kv, page, h, t0);
+            const HeadRows& from = value ? a.v : a.k;
+            const char* head = row_ptr(from, live ? row : sr.begin, h);
+            float y[NB][8];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) load8(head, from.type, true, 32 * b + 8 * g, y[b]);
+            if (!value && (a.w != nullptr || a.rope.table != nullptr)) {
+                double x[NB][8], scale = 1;
+                if (a.w != nullptr) {
+                    double sum = 0;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+                        for (int j = 0; j < 8; ++j) sum = __builtin_fma(static_cast<double>(y[b][j]), static_cast<double>(y[b][j]), sum);
+                    sum += __shfl_xor(sum, 16);
+                    sum += __shfl_xor(sum, 32);
+                    scale = 1.0 / sqrt(sum / HD + static_cast<double>(a.eps));
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    for (int j = 0; j < 8; ++j) {
+                        x[b][j] = y[b][j];
+                        if (a.w != nullptr) x[b][j] = x[b][j] * scale * static_cast<double>(a.w[32 * b + 8 * g + j]);
+                        y[b][j] = static_cast<float>(x[b][j]);
+                    }
+                }
+                if (a.rope.table != nullptr) {
+                    const float* cs = a.rope.table + static_cast<size_t>(live ? pos : 0) * a.rope.dims;
+                    const int dims = static_cast<int>(a.rope.dims);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const int d = 32 * b + 8 * g;
+                        if (!a.rope.neox) {
+                            if (d >= dims) continue;
+                            float t[8];
+                            load8(cs, kTypeF32, true, d, t);
+#pragma unroll
+                            for (int j = 0; j < 8; j += 2) {
+                                y[b][j] = static_cast<float>(mul_sub(x[b][j], static_cast<double>(t[j]), x[b][j + 1], static_cast<double>(t[j + 1])));
+                                y[b][j + 1] = static_cast<float>(mul_add(x[b][j], static_cast<double>(t[j + 1]), x[b][j + 1], static_cast<double>(t[j])));
+                            }
+                        } else {
+                            // dims / 64 blocks on: one of the lane's own, known when its number is
+#pragma unroll
+                            for (int o = 2 * b + 1; o < NB; ++o) {
+                                if (dims != 64 * (o - b)) continue;
+                                float t[16];
+                                load8(cs, kTypeF32, true, 2 * d, reinterpret_cast<float(&)[8]>(t[0]));
+                                load8(cs, kTypeF32, true, 2 * d + 8, reinterpret_cast<float(&)[8]>(t[8]));
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    const double c = t[2 * j], si = t[2 * j + 1];
+                                    y[b][j] = static_cast<float>(mul_sub(x[b][j], c, x[o][j], si));
+                                    y[o][j] = static_cast<float>(mul_add(x[b][j], si, x[o][j], c));
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            if constexpr (!Q4) {
+#pragma unroll
+                for (int n2 = 0; n2 < NG; ++n2) {
+                    uint32_t w[GS][4];
+#pragma unroll
+                    for (int e = 0; e < GS; ++e)
+                        for (int j = 0; j < 4; ++j) w[e][j] = pack_half(y[n2 * GS + e][2 * j], y[n2 * GS + e][2 * j + 1]);
+                    if (!live) continue;
+                    if (!value) {
+#pragma unroll
+                        for (int e = 0; e < GS; ++e) *reinterpret_cast<word4v*>(tile + ((n2 * GS + e) * 64 + lane) * 16) = word4v{w[e][0], w[e][1], w[e][2], w[e][3]};
+                    } else {
+                        uint8_t* to = tile + tile_values_at(false, NB) + ((i % 4 * NG + n2) * 64 + i / 4 * 16 + 4 * g) * GS * 4;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t z[GS];
+                            for (int e = 0; e < GS; ++e) z[e] = w[e][j];
+                            store_words<GS>(to + j * GS * 4, z);
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int n2 = 0; n2 < NG; ++n2) {
+                    uint32_t w[GS];
+#pragma unroll
+                    for (int e = 0; e < GS; ++e) {
+                        const int b = n2 * GS + e;
+                        uint32_t code[8];
+                        uint16_t scale;
+                        quantise8_tile(y[b], g, code, scale);
+                        w[e] = 0;
+                        for (int j = 0; j < 4; ++j)
+                            w[e] |= value ? (code[2 * j] | code[2 * j + 1] << 4) << (8 * j) : code[2 * j] << (4 * j) | code[2 * j + 1] << (4 * j + 16);
+                        if (live && g == b % 4) *reinterpret_cast<uint16_t*>(tile + scale_offset(NB, value, i, b)) = scale;
+                    }
+                    if (!value) {
+                        if (live) store_words<GS>(tile + (n2 * 64 + lane) * GS * 4, w);
+                    } else if (full) {
+#pragma unroll
+                        for (int e = 0; e < GS; ++e) w[e] = transposed(w[e], lane);
+                        store_words<GS>(tile + tile_values_at(true, NB) + (n2 * 64 + i / 4 * 16 + 4 * g + i % 4) * GS * 4, w);
+                    } else if (live) {
+#pragma unroll
+                        for (int e = 0; e < GS; ++e)
+                            for (int j = 0; j < 4; ++j)
+                                tile[value_offset(true, NB, i, 32 * (n2 * GS + e) + 8 * g + 2 * j)] = static_cast<uint8_t>(w[e] >> (8 * j));
+                    }
+                }
+            }
         }
     }
+}
+
+template <int NB>
+hipError_t launch_append(const AppendArgs& a, dim3 grid, hipStream_t st) {
+    if (a.kv.q4) k_kv_append_tiles<NB, true><<<grid, dim3(kThreads), 0, st>>>(a);
+    else k_kv_append_tiles<NB, false><<<grid, dim3(kThreads), 0, st>>>(a);
+    return hipGetLastError();
+}
+
+// One wave a tile's keys or values: loads of the whole tile, as the attention's.  A lane then has eight values of a
+// position (keys) or two of each of four (values), and 16 lanes write 64 bytes or more of a row.
+template <int NB, bool Q4>
+__global__ __launch_bounds__(kThreads) void k_kv_read(ReadArgs a, int vec) {
+    constexpr int GS = NB < 4 ? NB : 4, NG = NB / GS;
+    const int lane = static_cast<int>(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = lane % 16, g = lane / 16;
+    const uint32_t sides = a.k.data != nullptr && a.v.data != nullptr ? 2 : 1, units = a.pairs.d / 2 * sides;
+    for (uint32_t s = blockIdx.y; s < a.b.seqs; s += gridDim.y) {
+        const SeqRows sr = seq_rows(a.b, s);
+        if (sr.end <= sr.begin) continue;
+        const int32_t last = sr.first + (sr.end - sr.begin) - 1, t_lo = sr.first < 0 ? 0 : sr.first / 16, t_hi = last < 0 ? 0 : last / 16 + 1;
+        const uint32_t total = (t_hi - t_lo) * units;
+        for (uint32_t u = blockIdx.x * 4 + wave; u < total; u += gridDim.x * 4) {
+            const uint32_t n = sides == 2 ? over(u, a.pairs) : over(2 * u, a.pairs), rest = u - n * units;
+            const bool value = sides == 2 ? rest >= units / 2 : a.k.data == nullptr;
+            const uint32_t h = sides == 2 && value ? rest - units / 2 : rest;
+            const int32_t t0 = (t_lo + static_cast<int32_t>(n)) * 16, page = page_of(a.kv, a.b, s, t0);
+            if (page < 0) continue;
+            const uint8_t* tile = a.kv.data + tile_at(a.kv, page, h, t0);
+            const int32_t row0 = sr.begin + (t0 - sr.first);  // of the tile's first position; rows before sr.begin are not there
+            const HeadRows& y = value ? a.v : a.k;
+            const bool wide = vec & (value ? 2 : 1);
+            if (!value) {
+                const int32_t row = row0 + i;
+                const bool live = row >= sr.begin && row < sr.end;
+                char* out = row_ptr(y, live ? row : sr.begin, h);
+#pragma unroll
+                for (int m = 0; m < NG; ++m) {
+                    uint32_t w[GS];
+                    if constexpr (Q4) load_words<GS>(tile + (m * 64 + lane) * GS * 4, w);
+#pragma unroll
+                    for (int e = 0; e < GS; ++e) {
+                        const int b = m * GS + e;
+                        float x[8];
+                        if constexpr (Q4) {
+                            const float d = from_half(*reinterpret_cast<const uint16_t*>(tile + scale_offset(NB, false, i, b)));
+                            key_codes(w[e], d, x);
+                        } else {
+                            const word4v v = *reinterpret_cast<const word4v*>(tile + (b * 64 + lane) * 16);
+                            for (int j = 0; j < 4; ++j) {
+                                x[2 * j] = from_half(v[j] & 0xFFFF);
+                                x[2 * j + 1] = from_half(v[j] >> 16);
+                            }
+                        }
+                        if (live) store8(out, y.type, wide, 32 * b + 8 * g, x);
+                    }
+                }
+                continue;
+            }
+            const uint8_t* from = tile + tile_values_at(Q4, NB);
+#pragma unroll
+            for (int m = 0; m < NG; ++m) {
+                uint32_t w[Q4 ? 1 : 4][GS], d[Q4 ? 2 * GS : 1];
+                if constexpr (Q4) {
+                    load_words<GS>(from + (m * 64 + lane) * GS * 4, w[0]);
+                    load_words<2 * GS>(tile + tile_value_scales_at(NB) + (g * NB + m * GS) * 8, d);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) load_words<GS>(from + ((r * NG + m) * 64 + lane) * GS * 4, w[r]);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int32_t row = row0 + 4 * g + r;
+                    if (row < sr.begin || row >= sr.end) continue;
+                    char* out = row_ptr(y, row, h);
+#pragma unroll
+                    for (int e = 0; e < GS; ++e) {
+                        float x[2];
+                        if constexpr (Q4) {
+                            const uint32_t c = w[0][e] >> ((r & 1) * 16 + (r >> 1) * 8);
+                            const float f = from_half(d[2 * e + r / 2] >> (r % 2 * 16) & 0xFFFF);
+                            x[0] = (static_cast<float>(c & 15) - 8) * f;
+                            x[1] = (static_cast<float>(c >> 4 & 15) - 8) * f;
+                        } else {
+                            x[0] = from_half(w[r][e] & 0xFFFF);
+                            x[1] = from_half(w[r][e] >> 16);
+                        }
+                        store2(out, y.type, wide, 32 * (m * GS + e) + 2 * i, x);
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <int NB>
+hipError_t launch_read(const ReadArgs& a, dim3 grid, int vec, hipStream_t st) {
+    if (a.kv.q4) k_kv_read<NB, true><<<grid, dim3(kThreads), 0, st>>>(a, vec);
+    else k_kv_read<NB, false><<<grid, dim3(kThreads), 0, st>>>(a, vec);
+    return hipGetLastError();
+}
+
+// Blocks for the tiles that a sequence's rows may touch, a wave each for `units` of a tile.
+dim3 tile_grid(const PagedBatch& b, uint64_t units) {
+    const uint64_t most = b.max_rows == 0 || b.max_rows > b.rows ? b.rows : b.max_rows, tiles = (most + 14) / 16 + 1;
+    const uint64_t y = std::min<uint64_t>(b.seqs, 65535), x = std::min<uint64_t>((tiles * units + 3) / 4, std::max<uint64_t>(1, (1 << 18) / y));
+    return dim3(static_cast<uint32_t>(x), static_cast<uint32_t>(y));
 }
 
 // Blocks along a sequence's rows: enough for the largest, not many more than fill the card.
@@ -265,13 +533,25 @@ hipError_t launch_norm_rope(const NormRopeArgs& a, hipStream_t st) {
         if (a.x[t].data == nullptr) continue;
         vec |= (wide(a.x[t]) ? 1 << t : 0) | (wide(a.y[t]) ? 4 << t : 0);
     }
-    const size_t per = kThreads / lanes, total = a.n * (a.heads[0] + (a.x[1].data != nullptr ? a.heads[1] : 0));
+    const size_t per = kThreads / lanes, total = a.n * a.all.d;
     const size_t blocks = std::min<size_t>((total + per - 1) / per, 1 << 20);
     k_norm_rope<<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, st>>>(a, lanes, vec);
     return hipGetLastError();
 }
 
 hipError_t launch_kv_append(const AppendArgs& a, hipStream_t st) {
+    // By tiles where rows are read 16 bytes at a time and a rotation's pairs lie in one lane; otherwise row by row.
+    const bool turned_in_lane = a.rope.table == nullptr || (reinterpret_cast<uintptr_t>(a.rope.table) % 16 == 0 && a.rope.dims % (a.rope.neox ? 64 : 8) == 0);
+    if (wide(a.k) && wide(a.v) && turned_in_lane) {
+        const dim3 grid = tile_grid(a.b, a.pairs.d);
+        switch (a.kv.head_dim / 32) {
+            case 2: return launch_append<2>(a, grid, st);
+            case 3: return launch_append<3>(a, grid, st);
+            case 4: return launch_append<4>(a, grid, st);
+            case 8: return launch_append<8>(a, grid, st);
+            case 16: return launch_append<16>(a, grid, st);
+        }
+    }
     const int lanes = head_lanes(a.kv.head_dim);
     const int vec = (wide(a.k) ? 1 : 0) | (wide(a.v) ? 2 : 0);
     k_kv_append<<<row_grid(a.b, a.kv.kv_heads, lanes), dim3(kThreads), 0, st>>>(a, lanes, vec);
@@ -279,10 +559,16 @@ hipError_t launch_kv_append(const AppendArgs& a, hipStream_t st) {
 }
 
 hipError_t launch_kv_read(const ReadArgs& a, hipStream_t st) {
-    const int lanes = head_lanes(a.kv.head_dim);
     const int vec = (a.k.data != nullptr && wide(a.k) ? 1 : 0) | (a.v.data != nullptr && wide(a.v) ? 2 : 0);
-    k_kv_read<<<row_grid(a.b, a.kv.kv_heads, lanes), dim3(kThreads), 0, st>>>(a, lanes, vec);
-    return hipGetLastError();
+    const dim3 grid = tile_grid(a.b, static_cast<uint64_t>(a.kv.kv_heads) * (a.k.data != nullptr && a.v.data != nullptr ? 2 : 1));
+    switch (a.kv.head_dim / 32) {
+        case 2: return launch_read<2>(a, grid, vec, st);
+        case 3: return launch_read<3>(a, grid, vec, st);
+        case 4: return launch_read<4>(a, grid, vec, st);
+        case 8: return launch_read<8>(a, grid, vec, st);
+        case 16: return launch_read<16>(a, grid, vec, st);
+    }
+    return hipErrorInvalidValue;
 }
 
 }  // namespace bh

@@ -136,35 +136,39 @@ __device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {
     for (int k = 0; k < N; ++k) w[k] = x.w[k];
 }
 
-// Eight values of a position of a tile, from dimension d (a multiple of 8) on.
-__device__ inline void read8(const uint8_t* tile, bool q4, uint32_t nb, bool value, uint32_t token, uint32_t d, float (&x)[8]) {
-    if (!q4) {
-        uint32_t w[4];
-        if (!value) {
-            const word4v v = *reinterpret_cast<const word4v*>(tile + key_offset(false, nb, token, d));
-            for (int j = 0; j < 4; ++j) w[j] = v[j];
+template <int N, int ALIGN = N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4>
+__device__ inline void store_words(uint8_t* p, const uint32_t (&w)[N]) {
+    Words<N, ALIGN> x;
+    for (int k = 0; k < N; ++k) x.w[k] = w[k];
+    *reinterpret_cast<Words<N, ALIGN>*>(p) = x;
+}
+
+__device__ inline void store2(void* head, int type, bool vec, int d, const float (&x)[2]) {
+    if (type == kTypeF32) {
+        float* p = static_cast<float*>(head) + d;
+        if (vec) {
+            *reinterpret_cast<word2v*>(p) = word2v{__builtin_bit_cast(uint32_t, x[0]), __builtin_bit_cast(uint32_t, x[1])};
         } else {
-            for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint32_t*>(tile + value_offset(false, nb, token, d + 2 * j));
-        }
-        for (int j = 0; j < 4; ++j) {
-            x[2 * j] = from_half(w[j] & 0xFFFF);
-            x[2 * j + 1] = from_half(w[j] >> 16);
+            p[0] = x[0];
+            p[1] = x[1];
         }
         return;
     }
-    const float s = from_half(*reinterpret_cast<const uint16_t*>(tile + scale_offset(nb, value, token, d / 32)));
-    if (!value) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + key_offset(true, nb, token, d));
-        for (int m = 0; m < 4; ++m) {
-            x[2 * m] = (static_cast<float>(w >> (4 * m) & 15) - 8) * s;
-            x[2 * m + 1] = (static_cast<float>(w >> (4 * m + 16) & 15) - 8) * s;
-        }
+    const uint32_t lo = type == kTypeF16 ? to_half(x[0]) : to_bf16(x[0]), hi = type == kTypeF16 ? to_half(x[1]) : to_bf16(x[1]);
+    uint16_t* p = static_cast<uint16_t*>(head) + d;
+    if (vec) {
+        *reinterpret_cast<uint32_t*>(p) = lo | hi << 16;
     } else {
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t c = tile[value_offset(true, nb, token, d + 2 * j)];
-            x[2 * j] = (static_cast<float>(c & 15) - 8) * s;
-            x[2 * j + 1] = (static_cast<float>(c >> 4) - 8) * s;
-        }
+        p[0] = static_cast<uint16_t>(lo);
+        p[1] = static_cast<uint16_t>(hi);
+    }
+}
+
+// The eight keys of a word of codes.
+__device__ inline void key_codes(uint32_t w, float scale, float (&x)[8]) {
+    for (int m = 0; m < 4; ++m) {
+        x[2 * m] = (static_cast<float>(w >> (4 * m) & 15) - 8) * scale;
+        x[2 * m + 1] = (static_cast<float>(w >> (4 * m + 16) & 15) - 8) * scale;
     }
 }
 
