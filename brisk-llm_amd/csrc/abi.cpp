@@ -466,7 +466,6 @@ int brisk_hip_paged_attention(const brisk_hip_kv* kv, const brisk_hip_batch* bat
         if (need > workspace_bytes || (need != 0 && workspace == nullptr))
             bad("the attention needs " + std::to_string(need) + " bytes of workspace, and has " + std::to_string(workspace_bytes));
         if (need != 0 && reinterpret_cast<uintptr_t>(workspace) % 16 != 0) bad("the workspace is not 16-byte aligned");
-        a.splits = bh::paged_splits(a.kv, a.b, heads, a.q.type == bh::kTypeF32 || a.out.type == bh::kTypeF32);
         a.part = static_cast<float*>(workspace);
         hip_check(bh::launch_paged_attention(a, static_cast<hipStream_t>(stream)), "paged_attention");
     });

@@ -175,11 +175,11 @@ struct PagedAttnArgs {
     Divisor group, per_row, kv_heads;  // query heads of a key/value head, query heads, key/value heads
     float scale;
     uint32_t window;  // 0: none
-    uint32_t splits;
+    uint32_t splits;  // parts of the positions (set by the launcher, as `per`, the steps of one)
+    int32_t per;
     float* part;      // [rows][heads][splits][head_dim], then [rows][heads][splits][2] (maximum, sum)
 };
-// How many parts the positions are split into, and the workspace for them.
-uint32_t paged_splits(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bool exact);
+// The workspace for the parts that positions are split into.
 size_t paged_workspace(const PagedKv& kv, const PagedBatch& b, uint32_t heads);  // (for either precision)
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t st);
 // The prompts' kernel: the columns, (row, head) pairs of a key/value head, of its workgroup, and whether it takes a head size.

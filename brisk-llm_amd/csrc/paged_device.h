@@ -16,14 +16,35 @@ __device__ inline char* row_ptr(const HeadRows& x, int64_t row, int64_t head) {
     return static_cast<char*>(x.data) + (row * x.row + head * x.head) * (x.type == kTypeF32 ? 4 : 2);
 }
 
-// page_of for a position that is the same for the whole wave and not before 0, of a table that is not empty:
-// a scalar load and no branch.
-__device__ inline int32_t wave_page(const PagedKv& kv, const PagedBatch& b, uint32_t s, int32_t pos) {
-    const uint32_t e = static_cast<uint32_t>(pos) >> kv.page_shift, in = e < b.page_stride ? e : b.page_stride - 1;
+// A sequence's pages of one key/value head, for positions that are the same for the whole wave, not before 0, in a
+// table that is not empty: a scalar load and no branch.  Past the table's end the last entry is given: no row sees
+// such positions.
+struct WavePages {
     typedef const __attribute__((address_space(4))) int32_t* Table;
-    const int32_t p = ((Table)(uintptr_t)b.page_table)[static_cast<size_t>(s) * b.page_stride + in];
-    return e < b.page_stride && static_cast<uint32_t>(p) < kv.pages ? p : -1;
-}
+    Table table;
+    const uint8_t* head;  // the head's tiles of page 0
+    uint32_t last, shift, mask, pages, page_bytes;
+    __device__ inline WavePages(const PagedKv& kv, const PagedBatch& b, uint32_t s, uint32_t h) {
+        const uint32_t bytes = tile_bytes(kv.q4 != 0, kv.head_dim / 32), per = kv.page_tokens / kTileTokens;
+        table = (Table)(uintptr_t)(b.page_table + static_cast<size_t>(s) * b.page_stride);
+        last = b.page_stride - 1;
+        shift = kv.page_shift;
+        mask = kv.page_tokens - 1;
+        pages = kv.pages;
+        page_bytes = kv.kv_heads * per * bytes;  // (at most 2^31: 1024 heads of 64 tiles of 32 KB)
+        head = kv.data + static_cast<size_t>(h) * per * bytes;
+    }
+    // The page, or one past all pages.
+    __device__ inline uint32_t page(int32_t pos) const {
+        const uint32_t e = static_cast<uint32_t>(pos) >> shift;
+        return static_cast<uint32_t>(table[e < last ? e : last]);
+    }
+    __device__ inline bool there(uint32_t p) const { return p < pages; }
+    // The tile of a position of a page; of page 0 where there is none.
+    __device__ inline const uint8_t* tile(uint32_t p, int32_t pos, uint32_t bytes) const {
+        return head + static_cast<uint64_t>(p < pages ? p : 0) * page_bytes + (static_cast<uint32_t>(pos) & mask) / kTileTokens * bytes;
+    }
+};
 
 __device__ inline float from_bf16(uint32_t b) { return __builtin_bit_cast(float, b << 16); }
 __device__ inline float from_half(uint32_t h) { return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h))); }
@@ -91,6 +112,25 @@ constexpr float kLazy = 8.0f, kLift = 7.0f;
 __device__ inline float weight(float m, float next) {
     return __builtin_fmaxf(__builtin_amdgcn_exp2f(m - (next == -__builtin_inff() ? 0.0f : next)), 1.17549435e-38f);
 }
+
+// A column's running maximum: a raw score's, and times its scale.  A score's exponent is one fused operation, x scale -
+// base; for a scaled maximum past 2^20, whose rounding error would be an exponent of its own, the scores are
+// first moved by the maximum.
+struct Maximum {
+    float raw = -__builtin_inff(), m = -__builtin_inff(), base = 0, shift = 0;
+    bool far = false;  // whether some column of the wave is
+    // The factor of what has been summed, with a new score's maximum.
+    __device__ inline float renew(float top, float scale) {
+        raw = __builtin_fmaxf(raw, top);
+        const float next = raw * scale, f = weight(m, next);
+        m = next;
+        const bool none = m == -__builtin_inff(), mine = !none && __builtin_fabsf(m) > 1048576.0f;
+        shift = mine ? raw : 0.0f;
+        base = none ? 0.0f : mine ? -kLift : m - kLift;
+        far = __any(mine);
+        return f;
+    }
+};
 
 __device__ inline half8v operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(half8v, word4v{a, b, c, d}); }
 __device__ inline float4v mfma(half8v a, half8v b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }

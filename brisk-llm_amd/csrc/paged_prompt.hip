@@ -183,10 +183,11 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             bool there = false, poison = false;
             const int x = STEPS == 2 ? wave : wave & 3;
             const auto part = [&](int step) { return RawTile<NB, Q4>::first(STEPS == 2 ? step : wave >> 2); };
-            const auto page_at = [&](int32_t blk) { return wave_page(a.kv, a.b, s, blk * BLOCK + 16 * x); };
-            int32_t page = -1, page_next = -1;
+            const WavePages pages(a.kv, a.b, s, h);
+            const auto page_at = [&](int32_t blk) { return pages.page(blk * BLOCK + 16 * x); };
+            uint32_t page = 0, page_next = 0;
             const auto fetch = [&](int32_t blk, int step) {
-                raw[step].load(a.kv.data + tile_at(a.kv, page < 0 ? 0 : page, h, blk * BLOCK + 16 * x), part(step), lane);
+                raw[step].load(pages.tile(page, blk * BLOCK + 16 * x, tile_bytes(Q4, NB)), part(step), lane);
             };
             // some column does not see all of a block: what none sees is left out; and what is not finite
             const auto check = [&](int32_t blk) {
@@ -265,7 +266,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                             if constexpr (EXACT) *reinterpret_cast<half8v*>(&lds.q.part[1][wave][r][d]) = lo;
                         }
                     }
-                    if (sub == 0) lds.q.scale[wave][r] = __builtin_ldexpf(__builtin_fabsf(a.scale) * 1.44269504088896f, e - 9);
+                    // (never 0: scores of 0 and of minus infinity, what is not seen, stay what they are)
+                    if (sub == 0) lds.q.scale[wave][r] = __builtin_fmaxf(__builtin_ldexpf(__builtin_fabsf(a.scale) * 1.44269504088896f, e - 9), 1.17549435e-38f);
                 }
                 __builtin_amdgcn_wave_barrier();
                 if (col / 16 == c0 / 16) {
@@ -278,7 +280,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             }
             __syncthreads();  // (the queries' place is taken by the blocks)
 
-            float m = -__builtin_inff(), l = 0;
+            Maximum mx;
+            float l = 0;
             float16v acc[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) acc[b] = float16v{};
@@ -353,24 +356,28 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                     tops[x] = sc[x / 2][x % 2 * 8];
                     for (int r = 1; r < 8; ++r) tops[x] = __builtin_fmaxf(tops[x], sc[x / 2][x % 2 * 8 + r]);
                 }
-                float top = __builtin_fmaxf(__builtin_fmaxf(tops[0], tops[1]), __builtin_fmaxf(tops[2], tops[3])) * qscale;
-                if (__any(top > m + kLazy)) {
+                float top = __builtin_fmaxf(__builtin_fmaxf(tops[0], tops[1]), __builtin_fmaxf(tops[2], tops[3]));
+                if (__any(top * qscale > mx.m + kLazy)) {
                     top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-                    const float next = __builtin_fmaxf(m, top);
-                    const float f = weight(m, next);
-                    m = next;
+                    const float f = mx.renew(top, qscale);
                     l *= f;
 #pragma unroll
                     for (int b = 0; b < NB; ++b) acc[b] *= f;
                 }
-                const float base = m == -__builtin_inff() ? 0.0f : m - kLift;
+                if (mx.far) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        sc[0][r] -= mx.shift;
+                        sc[1][r] -= mx.shift;
+                    }
+                }
                 half8v p[PARTS][4];
                 float sums[2] = {};
                 const auto exponentials = [&](int tt) {
 #pragma unroll
                     for (int r = 0; r < 16; r += 2) {
-                        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[tt][r], qscale, -base));
-                        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[tt][r + 1], qscale, -base));
+                        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[tt][r], qscale, -mx.base));
+                        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[tt][r + 1], qscale, -mx.base));
                         const half2v e{static_cast<_Float16>(e0), static_cast<_Float16>(e1)};
                         p[0][2 * tt + r / 8][r % 8] = e[0];
                         p[0][2 * tt + r / 8][r % 8 + 1] = e[1];
@@ -417,13 +424,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                     // the values that are not finite, from the tiles themselves
 #pragma unroll 1
                     for (int u = 0; u < 4; ++u) {
-                        const int32_t t = t0 + 16 * u, page = wave_page(a.kv, a.b, s, t);
-                        const uint8_t* from = a.kv.data + tile_at(a.kv, page < 0 ? 0 : page, h, t);
+                        const int32_t t = t0 + 16 * u;
+                        const uint32_t at = pages.page(t);
+                        const uint8_t* from = pages.tile(at, t, tile_bytes(Q4, NB));
                         half8v sees;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const int32_t token = 16 * u + e / 4 * 8 + 4 * half + e % 4;
-                            sees[e] = static_cast<_Float16>(token <= hi && token > lo && page >= 0 ? 1.0f : 0.0f);
+                            sees[e] = static_cast<_Float16>(token <= hi && token > lo && pages.there(at) ? 1.0f : 0.0f);
                         }
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
@@ -446,7 +454,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             };
 
             if (blk_begin < blk_end) {
-                there = page >= 0;
+                there = pages.there(page);
                 check(blk_begin);
 #pragma unroll
                 for (int step = 0; step < STEPS; ++step) {
@@ -456,7 +464,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             }
             __syncthreads();
             for (int32_t blk = blk_begin; blk < blk_end; ++blk) {
-                there = page >= 0;
+                there = pages.there(page);
                 check(blk + 1);
 #pragma unroll
                 for (int step = 0; step < STEPS; ++step) {
@@ -478,7 +486,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 const uint32_t cc = tile * kWide + col, row = over(cc, a.group);
                 float* ml = a.part + static_cast<size_t>(a.b.rows) * a.heads * a.splits * HD +
                             ((static_cast<size_t>(sr.begin + row) * a.heads + h * a.group.d + (cc - row * a.group.d)) * a.splits + split) * 2;
-                ml[0] = m;
+                ml[0] = mx.m;
                 ml[1] = sum;
             }
 #pragma unroll 1

@@ -458,7 +458,7 @@ def test_attention_queries_that_are_not_finite_or_extreme(lib):
             q = rows(np.random.default_rng(2), 5, 2, 64, src)
             q[0, 0, 3], q[1, 1, 7] = float("inf"), float("nan")
             q[2] *= 1e30
-            q[3] *= 1e-30
+            q[3] *= 1e-38
             q[4] = 0
             q = q.cuda()
             out = cache.attend(q, 1.0)
@@ -471,6 +471,17 @@ def test_attention_queries_that_are_not_finite_or_extreme(lib):
             s = k[starts[2]:starts[2] + 50, 0] @ host(q)[2].T
             want = v[starts[2]:starts[2] + 50, 0][s.argmax(0)]  # one score far above the others
             assert (np.abs(got[2] - want) <= (2.0 ** -20 + (HALF_STEP[BF16] + 2.0 ** -10 if src == BF16 else 0)) * np.abs(want) + 1e-30).all()
+
+
+@pytest.mark.parametrize("rows_", [2, 200])
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-30])
+def test_attention_scales(lib, rows_, scale):
+    """No scale (the mean of what is seen), a negative one, one far below the products."""
+    for kind, src in ((F16, F16), (Q4_0, F32)):
+        batch = Batch([rows_], [300], 16)
+        cache = filled(lib, batch, kind, 2, 64)
+        q = rows(np.random.default_rng(2), rows_, 4, 64, src).cuda()
+        check_attention(cache, q, cache.attend(q, scale, 50), scale, 50)
 
 
 def test_attention_strides_types_and_broadcast(lib):
