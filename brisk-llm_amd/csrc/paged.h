@@ -183,7 +183,7 @@ struct PagedAttnArgs {
 size_t paged_workspace(const PagedKv& kv, const PagedBatch& b, uint32_t heads);  // (for either precision)
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t st);
 // The prompts' kernel: the columns, (row, head) pairs of a key/value head, of its workgroup, and whether it takes a head size.
-uint32_t prompt_columns();
+uint32_t prompt_columns(uint32_t head_dim, bool exact);
 bool prompt_fits(uint32_t head_dim, bool exact);
 hipError_t launch_paged_prompt(const PagedAttnArgs& a, bool exact, uint32_t max_rows, hipStream_t st);
 

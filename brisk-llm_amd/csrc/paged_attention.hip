@@ -602,7 +602,7 @@ hipError_t launch_sized(const PagedAttnArgs& a, dim3 grid, hipStream_t st) {
 
 // Prompts go to the kernel of many columns once those of a sequence fill half of its workgroup.
 bool is_prompt(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bool exact) {
-    return prompt_fits(kv.head_dim, exact) && static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads) * 2 >= prompt_columns();
+    return prompt_fits(kv.head_dim, exact) && static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads) * 2 >= prompt_columns(kv.head_dim, exact);
 }
 
 // The longest stretch of positions that a row's columns may see, as far as the host knows.
@@ -614,7 +614,7 @@ uint64_t longest(const PagedKv& kv, const PagedBatch& b, uint32_t window) {
 
 uint32_t paged_splits(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bool exact, uint32_t window) {
     const bool prompt = is_prompt(kv, b, heads, exact);
-    const uint64_t wide = prompt_columns(), cols = static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads);
+    const uint64_t wide = prompt_columns(kv.head_dim, exact), cols = static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads);
     const uint64_t blocks = static_cast<uint64_t>(b.seqs) * kv.kv_heads * (prompt ? (cols + wide - 1) / wide : column_tiles(kv, b, heads));
     // As many workgroups as are resident at once: each costs about 9 us before and after its positions.  Where there are
     // that many without, one for each 8192 positions, so that a long sequence among short ones does not run alone.

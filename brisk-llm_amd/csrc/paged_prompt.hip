@@ -13,10 +13,12 @@
 namespace bh {
 namespace {
 
-constexpr int kWaves = 8;
 constexpr int kBlock = 64;  // positions of a wave's step
 constexpr int kVector = 0x2, kMfma = 0x8;  // instructions' classes, for their order
 constexpr int kWide = 32;   // columns of a wave: (row, head) pairs of a key/value head
+
+// Waves of a workgroup, a CU's only one: two a SIMD where 256 registers hold a wave's queries and sums, otherwise one.
+constexpr int waves_of(int nb, bool exact) { return nb * (exact ? 2 : 1) <= 4 ? 8 : 4; }
 
 // What a thread holds of its wave's half of a tile, blocks b0 .. b0 + HB - 1 of every position, until it goes to LDS.
 template <int NB, bool Q4>
@@ -89,7 +91,7 @@ template <int NB, int PLANES, int STEPS>
 struct BlockLds {
     word4v k[PLANES][STEPS * 2][2 * NB][64];
     word4v v[PLANES][NB][STEPS * 4][64];
-    uint8_t there[kWaves], poison[kWaves];  // whether a wave's half tile is there, and holds values that are not finite (here they are zeros)
+    uint8_t there[8], poison[8];  // whether a wave's half tile is there, and holds values that are not finite (here they are zeros)
 };
 
 // A code times its scale, in one half (rounded: 2^-11 of the value at most, as the probabilities are), or in two (exact).
@@ -131,11 +133,12 @@ __device__ inline void unpack(const RawTile<NB, Q4>& raw, BlockLds<NB, PLANES, S
 // waves' columns are from the front of the prompt and half are their mirror image from the back: what
 // two such waves, which share a SIMD, see adds up to the same for all.
 template <int NB, bool Q4, bool EXACT>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_paged_prompt(PagedAttnArgs a) {
-    constexpr int HD = 32 * NB, PLANES = Q4 && EXACT ? 2 : 1, PARTS = EXACT ? 2 : 1;
-    // Two blocks in LDS, one multiplied while the other is filled: of 128 positions, a tile for each wave, where they fit
-    // (two 64-KB blocks), otherwise of 64, half a tile for each.
-    constexpr int STEPS = NB * PLANES <= 4 ? 2 : 1, BLOCK = STEPS * kBlock;
+__global__ __launch_bounds__(64 * waves_of(NB, EXACT)) __attribute__((amdgpu_waves_per_eu(waves_of(NB, EXACT) / 4, waves_of(NB, EXACT) / 4))) void k_paged_prompt(PagedAttnArgs a) {
+    constexpr int HD = 32 * NB, PLANES = Q4 && EXACT ? 2 : 1, PARTS = EXACT ? 2 : 1, kWaves = waves_of(NB, EXACT);
+    // Two blocks in LDS, one multiplied while the other is filled: of 128 positions for eight waves, where they fit
+    // (two 64-KB blocks), and of 64 for four: a tile for each wave.
+    constexpr int STEPS = kWaves / 4, BLOCK = STEPS * kBlock, HALVES = 2 / STEPS;
+    constexpr int CHUNK = NB < 4 ? 2 * NB : 8, CHUNKS = 4 * NB / CHUNK;  // operands that are read at a time
     typedef BlockLds<NB, PLANES, STEPS> Block;
     __shared__ union {
         Block block[2];
@@ -179,35 +182,36 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             const int32_t blk_begin = blk_lo + static_cast<int32_t>(std::min<int64_t>(blocks, static_cast<int64_t>(per) * split));
             const int32_t blk_end = blk_lo + static_cast<int32_t>(std::min<int64_t>(blocks, static_cast<int64_t>(per) * (split + 1)));
 
-            RawTile<NB, Q4> raw[STEPS];
+            RawTile<NB, Q4> raw[2];  // the wave's tile of a block, in halves: one for each step, or both for the only one
             bool there = false, poison = false;
-            const int x = STEPS == 2 ? wave : wave & 3;
-            const auto part = [&](int step) { return RawTile<NB, Q4>::first(STEPS == 2 ? step : wave >> 2); };
+            const auto part = [&](int n) { return RawTile<NB, Q4>::first(n); };
             const WavePages pages(a.kv, a.b, s, h);
-            const auto page_at = [&](int32_t blk) { return pages.page(blk * BLOCK + 16 * x); };
+            const auto page_at = [&](int32_t blk) { return pages.page(blk * BLOCK + 16 * wave); };
             uint32_t page = 0, page_next = 0;
             const auto fetch = [&](int32_t blk, int step) {
-                raw[step].load(pages.tile(page, blk * BLOCK + 16 * x, tile_bytes(Q4, NB)), part(step), lane);
+#pragma unroll
+                for (int n = step * HALVES; n < (step + 1) * HALVES; ++n) raw[n].load(pages.tile(page, blk * BLOCK + 16 * wave, tile_bytes(Q4, NB)), part(n), lane);
             };
             // some column does not see all of a block: what none sees is left out; and what is not finite
             const auto check = [&](int32_t blk) {
                 if (!there || (blk + 1) * BLOCK - 1 > wg_plo || (window != 0 && blk * BLOCK <= wg_phi - window)) {
-                    const int32_t t = blk * BLOCK + 16 * x + 4 * (lane / 16);
+                    const int32_t t = blk * BLOCK + 16 * wave + 4 * (lane / 16);
                     uint32_t keep = 0;
                     for (int r = 0; r < 4; ++r) keep |= there && t + r >= wg_lo && t + r <= wg_phi ? 1u << r : 0;
 #pragma unroll
-                    for (int step = 0; step < STEPS; ++step) raw[step].keep_values(keep);
+                    for (int n = 0; n < 2; ++n) raw[n].keep_values(keep);
                 }
                 poison = raw[0].any_ill();
-                if constexpr (STEPS == 2) poison |= raw[1].any_ill();
+                poison |= raw[1].any_ill();
                 if (__builtin_expect(poison, 0)) {
 #pragma unroll
-                    for (int step = 0; step < STEPS; ++step) raw[step].drop_ill();
+                    for (int n = 0; n < 2; ++n) raw[n].drop_ill();
                 }
             };
-            const auto put = [&](int32_t blk, int step) {
+            const auto put = [&](int32_t blk, int n0, int count) {
                 Block& out = lds.block[blk & 1];
-                unpack<NB, Q4, PLANES, STEPS>(raw[step], out, x, part(step), lane);
+#pragma unroll
+                for (int n = n0; n < n0 + count; ++n) unpack<NB, Q4, PLANES, STEPS>(raw[n], out, wave, part(n), lane);
                 out.there[wave] = there;  // (every lane the same: a branch would end the block of instructions that is scheduled)
                 out.poison[wave] = poison;
             };
@@ -291,51 +295,64 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             const auto sub = [&](const Block& in, int32_t blk, int step) {
                 const int32_t t0 = blk * BLOCK + step * kBlock;
                 const uint32_t heres = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(in.there)[step]);
-                const uint32_t* ill_at = reinterpret_cast<const uint32_t*>(in.poison);
-                const uint32_t ills = __builtin_amdgcn_readfirstlane(STEPS == 2 ? ill_at[step] : ill_at[0] | ill_at[1]);
+                const uint32_t ills = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(in.poison)[step]);
                 float16v sc[2] = {};
-                // The operands of half of the steps are read ahead of the products of the other half; the
-                // barriers keep the compiler from undoing that.
-                const auto read_keys = [&](half8v (&x)[PLANES][2 * NB], int k0) {
+                // A chunk's operands are read ahead of the products of the chunk before; the barriers keep the compiler
+                // from undoing that.
+                half8v ops[2][PLANES][CHUNK];
+                const auto read_keys = [&](int c) {
 #pragma unroll
-                    for (int k = 0; k < 2 * NB; ++k)
-                        for (int e = 0; e < PLANES; ++e) x[e][k] = __builtin_bit_cast(half8v, in.k[e][2 * step + k % 2][k0 + k / 2][lane]);
+                    for (int k = 0; k < CHUNK; ++k)
+                        for (int e = 0; e < PLANES; ++e) ops[c % 2][e][k] = __builtin_bit_cast(half8v, in.k[e][2 * step + k % 2][c * CHUNK / 2 + k / 2][lane]);
                 };
-                const auto keys_times = [&](const half8v (&x)[PLANES][2 * NB], int k0) {
+                const auto keys_times = [&](int c) {
 #pragma unroll
-                    for (int k = 0; k < 2 * NB; ++k) {
+                    for (int k = 0; k < CHUNK; ++k) {
+                        const int at = c * CHUNK / 2 + k / 2;
                         if constexpr (EXACT) {
-                            sc[k % 2] = mfma(x[0][k], q[1][k0 + k / 2], sc[k % 2]);
-                            if constexpr (Q4) sc[k % 2] = mfma(x[1][k], q[0][k0 + k / 2], sc[k % 2]);
+                            sc[k % 2] = mfma(ops[c % 2][0][k], q[1][at], sc[k % 2]);
+                            if constexpr (Q4) sc[k % 2] = mfma(ops[c % 2][1][k], q[0][at], sc[k % 2]);
                         }
-                        sc[k % 2] = mfma(x[0][k], q[0][k0 + k / 2], sc[k % 2]);
+                        sc[k % 2] = mfma(ops[c % 2][0][k], q[0][at], sc[k % 2]);
                     }
                 };
-                half8v ops[2][PLANES][2 * NB];
-                read_keys(ops[0], 0);
-                __builtin_amdgcn_sched_barrier(0);
-                read_keys(ops[1], NB);
-                __builtin_amdgcn_sched_barrier(0);
-                put(blk + 1, step);
-                keys_times(ops[0], 0);
-                keys_times(ops[1], NB);
-                if constexpr (!EXACT) {
+                read_keys(0);
 #pragma unroll
-                    for (int k = 0; k < 4 * NB; ++k) {
-                        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(kVector, 4, 0);
+                for (int c = 0; c < CHUNKS; c += 2) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    read_keys(c + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (CHUNKS == 2) put(blk + 1, step * HALVES, HALVES);
+                    else put(blk + 1, c / 2, 1);
+                    keys_times(c);
+                    if constexpr (CHUNKS != 2) {
+#pragma unroll
+                        for (int k = 0; k < CHUNK; ++k) {
+                            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(kVector, 16, 0);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (c + 2 < CHUNKS) read_keys(c + 2);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    keys_times(c + 1);
+                    if constexpr (CHUNKS == 2 && !EXACT) {
+#pragma unroll
+                        for (int k = 0; k < 4 * NB; ++k) {
+                            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(kVector, 4, 0);
+                        }
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 next(blk, step);
-                // the values' operands likewise, of 32 positions at a time
-                const auto read_values = [&](half8v (&x)[PLANES][2 * NB], int u0) {
+                // the values' operands likewise
+                const auto read_values = [&](int c) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        for (int b = 0; b < NB; ++b)
-                            for (int e = 0; e < PLANES; ++e) x[e][u * NB + b] = __builtin_bit_cast(half8v, in.v[e][b][4 * step + u0 + u][lane]);
+                    for (int k = 0; k < CHUNK; ++k)
+                        for (int e = 0; e < PLANES; ++e) ops[c % 2][e][k] = __builtin_bit_cast(half8v, in.v[e][k % NB][4 * step + c * (CHUNK / NB) + k / NB][lane]);
                 };
-                read_values(ops[0], 0);
+                read_values(0);
                 __builtin_amdgcn_sched_barrier(0);
                 // the column sees positions t0 + u with lo < u <= hi, in tiles that are there
                 const int32_t hi = pos - t0, lo = window != 0 ? hi - window : -1;
@@ -391,34 +408,35 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                         }
                     }
                 };
-                const auto values_times = [&](const half8v (&x)[PLANES][2 * NB], int u0) {
+                const auto values_times = [&](int c) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            if constexpr (EXACT) {
-                                acc[b] = mfma(x[0][u * NB + b], p[1][u0 + u], acc[b]);
-                                if constexpr (Q4) acc[b] = mfma(x[1][u * NB + b], p[0][u0 + u], acc[b]);
-                            }
-                            acc[b] = mfma(x[0][u * NB + b], p[0][u0 + u], acc[b]);
+                    for (int k = 0; k < CHUNK; ++k) {
+                        const int u = c * (CHUNK / NB) + k / NB, b = k % NB;
+                        if constexpr (EXACT) {
+                            acc[b] = mfma(ops[c % 2][0][k], p[1][u], acc[b]);
+                            if constexpr (Q4) acc[b] = mfma(ops[c % 2][1][k], p[0][u], acc[b]);
                         }
+                        acc[b] = mfma(ops[c % 2][0][k], p[0][u], acc[b]);
                     }
                 };
                 exponentials(0);
-                __builtin_amdgcn_sched_barrier(0);
-                read_values(ops[1], 2);
-                __builtin_amdgcn_sched_barrier(0);
-                values_times(ops[0], 0);
-                exponentials(1);
-                if constexpr (!EXACT) {  // the second exponentials under the first products
 #pragma unroll
-                    for (int k = 0; k < 2 * NB; ++k) {
-                        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(kVector, 24 / NB, 0);
+                for (int c = 0; c < CHUNKS; ++c) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (c + 1 < CHUNKS) read_values(c + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    values_times(c);
+                    if (c == 0) {  // the second exponentials under the first products
+                        exponentials(1);
+                        if constexpr (!EXACT) {
+#pragma unroll
+                            for (int k = 0; k < CHUNK; ++k) {
+                                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                                __builtin_amdgcn_sched_group_barrier(kVector, 48 / CHUNK, 0);
+                            }
+                        }
                     }
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                values_times(ops[1], 2);
                 l += sums[0] + sums[1];
                 if (__builtin_expect(ills != 0, 0)) {
                     // the values that are not finite, from the tiles themselves
@@ -458,7 +476,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 check(blk_begin);
 #pragma unroll
                 for (int step = 0; step < STEPS; ++step) {
-                    put(blk_begin, step);
+                    put(blk_begin, step * HALVES, HALVES);
                     next(blk_begin - 1, step);
                 }
             }
@@ -472,7 +490,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                     if (t0 < t_hi && t0 + kBlock > t_lo) {
                         sub(lds.block[blk & 1], blk, step);
                     } else {
-                        put(blk + 1, step);
+                        put(blk + 1, step * HALVES, HALVES);
                         next(blk, step);
                     }
                 }
@@ -526,7 +544,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 
 template <int NB>
 hipError_t launch_typed(const PagedAttnArgs& a, bool exact, dim3 grid, hipStream_t st) {
-    const dim3 threads(64 * kWaves);
+    const dim3 threads(64 * waves_of(NB, exact));
     if (!exact) {
         if (a.kv.q4) k_paged_prompt<NB, true, false><<<grid, threads, 0, st>>>(a);
         else k_paged_prompt<NB, false, false><<<grid, threads, 0, st>>>(a);
@@ -541,13 +559,13 @@ hipError_t launch_typed(const PagedAttnArgs& a, bool exact, dim3 grid, hipStream
 
 }  // namespace
 
-uint32_t prompt_columns() { return kWide * kWaves; }
+uint32_t prompt_columns(uint32_t head_dim, bool exact) { return kWide * waves_of(static_cast<int>(head_dim / 32), exact); }
 
 // 32-bit results take twice the registers and, of 4-bit caches, twice the LDS: heads of up to 128 values.
 bool prompt_fits(uint32_t head_dim, bool exact) { return head_dim <= (exact ? 128 : 256); }
 
 hipError_t launch_paged_prompt(const PagedAttnArgs& a, bool exact, uint32_t max_rows, hipStream_t st) {
-    const uint32_t wide = prompt_columns();
+    const uint32_t wide = prompt_columns(a.kv.head_dim, exact);
     const uint64_t cols = static_cast<uint64_t>(max_rows) * a.group.d, sets = std::min<uint64_t>((cols + wide - 1) / wide, 65535 / a.splits);
     const dim3 grid(a.kv.kv_heads, static_cast<uint32_t>(sets * a.splits), std::min<uint32_t>(a.b.seqs, 65535));
     switch (a.kv.head_dim / 32) {
