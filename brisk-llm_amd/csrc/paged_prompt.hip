@@ -134,7 +134,7 @@ __device__ inline void unpack(const RawTile<NB, Q4>& raw, BlockLds<NB, PLANES, S
 // two such waves, which share a SIMD, see adds up to the same for all.
 template <int NB, bool Q4, bool EXACT>
 __global__ __launch_bounds__(64 * waves_of(NB, EXACT)) __attribute__((amdgpu_waves_per_eu(waves_of(NB, EXACT) / 4, waves_of(NB, EXACT) / 4))) void k_paged_prompt(PagedAttnArgs a) {
-    constexpr int HD = 32 * NB, PLANES = Q4 && EXACT ? 2 : 1, PARTS = EXACT ? 2 : 1, kWaves = waves_of(NB, EXACT);
+    constexpr int HD = 32 * NB, PLANES = Q4 && EXACT ? 2 : 1, PARTS = EXACT ? 2 : 1, PRODUCTS = EXACT + PLANES, kWaves = waves_of(NB, EXACT);
     // Two blocks in LDS, one multiplied while the other is filled: of 128 positions for eight waves, where they fit
     // (two 64-KB blocks), and of 64 for four: a tile for each wave.
     constexpr int STEPS = kWaves / 4, BLOCK = STEPS * kBlock, HALVES = 2 / STEPS;
@@ -336,11 +336,11 @@ __global__ __launch_bounds__(64 * waves_of(NB, EXACT)) __attribute__((amdgpu_wav
                         __builtin_amdgcn_sched_barrier(0);
                     }
                     keys_times(c + 1);
-                    if constexpr (CHUNKS == 2 && !EXACT) {
+                    if constexpr (CHUNKS == 2) {
 #pragma unroll
-                        for (int k = 0; k < 4 * NB; ++k) {
+                        for (int k = 0; k < 4 * NB * PRODUCTS; ++k) {
                             __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-                            __builtin_amdgcn_sched_group_barrier(kVector, 4, 0);
+                            __builtin_amdgcn_sched_group_barrier(kVector, EXACT ? 6 : 4, 0);
                         }
                     }
                 }
@@ -428,12 +428,10 @@ __global__ __launch_bounds__(64 * waves_of(NB, EXACT)) __attribute__((amdgpu_wav
                     values_times(c);
                     if (c == 0) {  // the second exponentials under the first products
                         exponentials(1);
-                        if constexpr (!EXACT) {
 #pragma unroll
-                            for (int k = 0; k < CHUNK; ++k) {
-                                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-                                __builtin_amdgcn_sched_group_barrier(kVector, 48 / CHUNK, 0);
-                            }
+                        for (int k = 0; k < CHUNK * PRODUCTS; ++k) {
+                            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(kVector, 48 / CHUNK, 0);
                         }
                     }
                 }
