@@ -600,11 +600,6 @@ hipError_t launch_sized(const PagedAttnArgs& a, dim3 grid, hipStream_t st) {
 
 }  // namespace
 
-// Prompts go to the kernel of many columns once those of a sequence fill half of its workgroup.
-bool is_prompt(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bool exact) {
-    return prompt_fits(kv.head_dim, exact) && static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads) * 2 >= prompt_columns(kv.head_dim, exact);
-}
-
 // The longest stretch of positions that a row's columns may see, as far as the host knows.
 uint64_t longest(const PagedKv& kv, const PagedBatch& b, uint32_t window) {
     const uint64_t capacity = static_cast<uint64_t>(b.page_stride) * kv.page_tokens;
@@ -612,15 +607,29 @@ uint64_t longest(const PagedKv& kv, const PagedBatch& b, uint32_t window) {
     return window == 0 ? length : std::min<uint64_t>(length, static_cast<uint64_t>(window) + most_rows(b));
 }
 
+// Prompts go to the kernel of many columns where those of a sequence fill half of its workgroup and there is enough to
+// do: its workgroups start slowly (25 to 50 us), and 16 columns' fill the card at once.  Measured here and there, in us
+// (without a window, since the workspace is sized before it is known): 128 rows of 8000 positions, 16 heads of 128
+// in 4 bits 57 and 40, 300 rows 95 and 106; 100 rows of 20000, 32 heads of 64 64 and 90; 1500 rows of 1500 57 and 51;
+// 1000 rows of 4000, 8 heads of 256 93 and 93; 32-bit, 1000 rows of 3000, 16 heads of 128 88 and 71.
+bool is_prompt(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bool exact) {
+    const uint64_t length = longest(kv, b, 0), seen = length - std::min<uint64_t>(length, most_rows(b)) / 2;  // on average
+    const double work = static_cast<double>(b.rows) * heads * kv.head_dim * static_cast<double>(seen);
+    return prompt_fits(kv.head_dim, exact) && work >= (exact ? 7e9 : 3.5e9) &&
+           static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads) * 2 >= prompt_columns(kv.head_dim, exact);
+}
+
 uint32_t paged_splits(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bool exact, uint32_t window) {
     const bool prompt = is_prompt(kv, b, heads, exact);
     const uint64_t wide = prompt_columns(kv.head_dim, exact), cols = static_cast<uint64_t>(most_rows(b)) * (heads / kv.kv_heads);
     const uint64_t blocks = static_cast<uint64_t>(b.seqs) * kv.kv_heads * (prompt ? (cols + wide - 1) / wide : column_tiles(kv, b, heads));
     // As many workgroups as are resident at once: each costs about 9 us before and after its positions.  Where there are
-    // that many without, one for each 8192 positions, so that a long sequence among short ones does not run alone.
+    // that many without, one for each 8192 positions, so that a long sequence among short ones does not run alone, of
+    // 256 MB at most.
     const uint64_t target = 256 * resident(static_cast<int>(kv.head_dim / 32)), most = longest(kv, b, window);
     const uint64_t least = prompt ? 512 : kWaves * step_of(kv), useful = (most + least - 1) / least;
-    const uint64_t wanted = prompt ? 256 / blocks : std::max<uint64_t>(target / blocks, (most + 8191) / 8192);
+    const uint64_t room = (uint64_t{1} << 26) / (std::max<uint64_t>(b.rows, 1) * heads * (kv.head_dim + 2));
+    const uint64_t wanted = prompt ? 256 / blocks : std::max<uint64_t>(target / blocks, std::min<uint64_t>((most + 8191) / 8192, room));
     return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(std::min(useful, wanted), kMaxSplits)));
 }
 

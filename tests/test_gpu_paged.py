@@ -34,6 +34,15 @@ def lib():
     return L.load()
 
 
+@pytest.fixture(params=["lengths", "wide"])
+def tables(request):
+    """The host knows the lengths, or only that the tables have room for 2^20 positions: then there are more parts, and
+    prompts go to the kernel of many columns."""
+    Cache.wide_tables = request.param == "wide"
+    yield
+    Cache.wide_tables = False
+
+
 def heads_of(x):
     return L.HipHeads(x.data_ptr(), {v: k for k, v in TORCH.items()}[x.dtype], x.stride(0), x.stride(1))
 
@@ -61,6 +70,7 @@ def host(t):
 
 class Cache:
     """A cache and a batch on the GPU.  The cache's bytes start as 0xFF, which read as NaN."""
+    wide_tables = False
 
     def __init__(self, lib, batch, kind, kv_heads, dim, max_rows=None, max_length=None, extra_rows=0):
         self.lib, self.batch, self.kind = lib, batch, kind
@@ -76,8 +86,12 @@ class Cache:
 
     def set(self, batch):
         self.batch = batch
-        self.arrays = [torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).cuda() for a in (batch.starts, batch.lengths, batch.table)]
-        self.b = L.HipBatch(*[a.data_ptr() for a in self.arrays], len(batch.rows), batch.n + self.extra, batch.stride, self.max_rows, self.max_length)
+        table, length = batch.table, self.max_length
+        if Cache.wide_tables:
+            table, length = np.pad(table, ((0, 0), (0, (1 << 20) // batch.page - table.shape[1])), constant_values=-1), 0
+        self.arrays = [torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).cuda() for a in (batch.starts, batch.lengths, table)]
+        stride = table.shape[1] if Cache.wide_tables else batch.stride
+        self.b = L.HipBatch(*[a.data_ptr() for a in self.arrays], len(batch.rows), batch.n + self.extra, stride, self.max_rows, length)
 
     def append(self, k, v, w=None, eps=1e-6, rope=None):
         kh, vh = heads_of(k), heads_of(v)
@@ -333,6 +347,7 @@ def filled(lib, batch, kind, kvh, dim, seed=0, **more):
 LENGTHS = [([1, 1, 1, 1], [1, 17, 700, 1300]), ([3, 8, 1], [40, 8, 333]), ([70, 33], [200, 33]), ([300, 1, 0, 129], [300, 500, 70, 700])]
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("rows_,lengths", LENGTHS, ids=["tokens", "drafted", "prompts", "mixed"])
 @pytest.mark.parametrize("kind", [F16, Q4_0], ids=NAMES.get)
 @pytest.mark.parametrize("heads,kvh,dim,src", [(16, 8, 128, F16), (4, 1, 64, BF16), (6, 2, 96, F32), (4, 1, 256, F32), (8, 2, 256, F16), (8, 1, 512, F32),
@@ -356,6 +371,7 @@ def test_attention_long(lib, kind, src):
     check_attention(cache, q, cache.attend(q, 0.0884), 0.0884, 0)
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("kind", [F16, Q4_0], ids=NAMES.get)
 @pytest.mark.parametrize("rows_", [[1, 4, 9, 0, 2], [30, 64, 50, 0, 40]], ids=["few", "many"])
 def test_attention_rows_that_see_nothing(lib, kind, rows_):
@@ -374,6 +390,7 @@ def test_attention_rows_that_see_nothing(lib, kind, rows_):
     check_attention(cache, q, out, 0.125, 3)
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("kind", [F16, Q4_0], ids=NAMES.get)
 @pytest.mark.parametrize("src", [F16, F32], ids=NAMES.get)
 @pytest.mark.parametrize("rows_", [3, 40])
@@ -402,6 +419,7 @@ def test_attention_does_not_depend_on_the_hosts_bounds(lib, hints):
     check_attention(cache, q, cache.attend(q, 0.125), 0.125, 0)
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("kind", [F16, Q4_0], ids=NAMES.get)
 @pytest.mark.parametrize("src", [F16, F32], ids=NAMES.get)
 @pytest.mark.parametrize("rows_", [6, 60])
@@ -429,6 +447,7 @@ def test_attention_values_that_are_not_finite(lib, kind, src, rows_, window):
     assert not np.isfinite(got[-1]).any()  # a NaN key: its row's every value
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("src", [F16, F32], ids=NAMES.get)
 @pytest.mark.parametrize("rows_", [1, 200])
 def test_attention_infinity_with_a_small_probability(lib, src, rows_):
@@ -473,6 +492,7 @@ def test_attention_queries_that_are_not_finite_or_extreme(lib):
             assert (np.abs(got[2] - want) <= (2.0 ** -20 + (HALF_STEP[BF16] + 2.0 ** -10 if src == BF16 else 0)) * np.abs(want) + 1e-30).all()
 
 
+@pytest.mark.usefixtures("tables")
 @pytest.mark.parametrize("rows_", [2, 200])
 @pytest.mark.parametrize("scale", [0.0, -0.125, 1e-30])
 def test_attention_scales(lib, rows_, scale):
@@ -484,6 +504,7 @@ def test_attention_scales(lib, rows_, scale):
         check_attention(cache, q, cache.attend(q, scale, 50), scale, 50)
 
 
+@pytest.mark.usefixtures("tables")
 def test_attention_strides_types_and_broadcast(lib):
     """Queries inside fused rows, outputs by head, 32-bit outputs of 16-bit queries and the other way round, one query for all heads."""
     batch = Batch([2, 30], [300, 60], 32)
