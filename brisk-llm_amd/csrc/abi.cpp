@@ -429,7 +429,8 @@ int brisk_hip_kv_read(const brisk_hip_kv* kv, const brisk_hip_batch* batch, cons
         if (k != nullptr) a.k = written_rows(k, "keys", a.b.rows, a.kv.kv_heads, a.kv.head_dim);
         if (v != nullptr) a.v = written_rows(v, "values", a.b.rows, a.kv.kv_heads, a.kv.head_dim);
         if (k == nullptr && v == nullptr) return;
-        a.pairs = cache_pairs(a.kv, a.b);
+        (void)cache_pairs(a.kv, a.b);
+        a.heads = bh::divisor(a.kv.kv_heads);
         hip_check(bh::launch_kv_read(a, static_cast<hipStream_t>(stream)), "kv_read");
     });
 }

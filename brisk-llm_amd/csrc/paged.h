@@ -163,7 +163,7 @@ struct ReadArgs {
     PagedKv kv;
     PagedBatch b;
     HeadRows k, v;  // data null: not wanted
-    Divisor pairs;  // 2 x key/value heads
+    Divisor heads;  // key/value heads
 };
 hipError_t launch_kv_read(const ReadArgs& a, hipStream_t st);
 

@@ -416,85 +416,94 @@ hipError_t launch_append(const AppendArgs& a, dim3 grid, hipStream_t st) {
     return hipGetLastError();
 }
 
-// One wave a tile's keys or values: loads of the whole tile, as the attention's.  A lane then has eight values of a
-// position (keys) or two of each of four (values), and 16 lanes write 64 bytes or more of a row.
+// The inverse of transposed(): a word's positions in the order 0, 2, 1, 3 go to the four lanes, in the order of the dimensions.
+__device__ inline uint32_t untransposed(uint32_t w, int lane) {
+    w = transposed(__builtin_amdgcn_perm(0, w, 0x03010200), lane);
+    return __builtin_amdgcn_perm(0, w, 0x03010200);
+}
+
+// A 4 x 4 transposition of words in each four lanes: lane j's word q goes to lane q's word j.
+__device__ inline void transpose_words(uint32_t (&x)[4], int lane) {
+    for (int r = 0; r < 4; r += 2) {
+        const uint32_t t = __builtin_amdgcn_update_dpp(0, lane & 1 ? x[r] : x[r + 1], 0xB1, 0xF, 0xF, true);
+        (lane & 1 ? x[r] : x[r + 1]) = t;
+    }
+    for (int r = 0; r < 2; ++r) {
+        const uint32_t t = __builtin_amdgcn_update_dpp(0, lane & 2 ? x[r] : x[r + 2], 0x4E, 0xF, 0xF, true);
+        (lane & 2 ? x[r] : x[r + 2]) = t;
+    }
+}
+
+// One wave a tile: loads of the whole of it, as the attention's, keys' and values' on their way together.  A lane
+// then has eight values of a position, of values after a transposition among four lanes, and four lanes write 64 bytes or
+// more of a row, past the caches: 4 sequences of 16000 positions, 8 heads of 128 in 4 bits to fp16, take 56 us, as long as a
+// copy of as many bytes (5.2 TB/s), and through the caches 86.
 template <int NB, bool Q4>
 __global__ __launch_bounds__(kThreads) void k_kv_read(ReadArgs a, int vec) {
     constexpr int GS = NB < 4 ? NB : 4, NG = NB / GS;
     const int lane = static_cast<int>(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = lane % 16, g = lane / 16;
-    const uint32_t sides = a.k.data != nullptr && a.v.data != nullptr ? 2 : 1, units = a.pairs.d / 2 * sides;
     for (uint32_t s = blockIdx.y; s < a.b.seqs; s += gridDim.y) {
         const SeqRows sr = seq_rows(a.b, s);
         if (sr.end <= sr.begin) continue;
         const int32_t last = sr.first + (sr.end - sr.begin) - 1, t_lo = sr.first < 0 ? 0 : sr.first / 16, t_hi = last < 0 ? 0 : last / 16 + 1;
-        const uint32_t total = (t_hi - t_lo) * units;
+        const uint32_t total = (t_hi - t_lo) * a.heads.d;
         for (uint32_t u = blockIdx.x * 4 + wave; u < total; u += gridDim.x * 4) {
-            const uint32_t n = sides == 2 ? over(u, a.pairs) : over(2 * u, a.pairs), rest = u - n * units;
-            const bool value = sides == 2 ? rest >= units / 2 : a.k.data == nullptr;
-            const uint32_t h = sides == 2 && value ? rest - units / 2 : rest;
+            const uint32_t n = over(u, a.heads), h = u - n * a.heads.d;
             const int32_t t0 = (t_lo + static_cast<int32_t>(n)) * 16, page = page_of(a.kv, a.b, s, t0);
             if (page < 0) continue;
-            const uint8_t* tile = a.kv.data + tile_at(a.kv, page, h, t0);
-            const int32_t row0 = sr.begin + (t0 - sr.first);  // of the tile's first position; rows before sr.begin are not there
-            const HeadRows& y = value ? a.v : a.k;
-            const bool wide = vec & (value ? 2 : 1);
-            if (!value) {
-                const int32_t row = row0 + i;
-                const bool live = row >= sr.begin && row < sr.end;
-                char* out = row_ptr(y, live ? row : sr.begin, h);
+            const uint8_t *tile = a.kv.data + tile_at(a.kv, page, h, t0), *from = tile + tile_values_at(Q4, NB);
+            uint32_t k[NG][Q4 ? 1 : GS][Q4 ? GS : 4], v[NG][Q4 ? 1 : 4][GS], vs[NG][Q4 ? 2 * GS : 1];
+            uint16_t ks[Q4 ? NB : 1];
+            if (a.k.data != nullptr) {
 #pragma unroll
                 for (int m = 0; m < NG; ++m) {
-                    uint32_t w[GS];
-                    if constexpr (Q4) load_words<GS>(tile + (m * 64 + lane) * GS * 4, w);
-#pragma unroll
-                    for (int e = 0; e < GS; ++e) {
-                        const int b = m * GS + e;
-                        float x[8];
-                        if constexpr (Q4) {
-                            const float d = from_half(*reinterpret_cast<const uint16_t*>(tile + scale_offset(NB, false, i, b)));
-                            key_codes(w[e], d, x);
-                        } else {
-                            const word4v v = *reinterpret_cast<const word4v*>(tile + (b * 64 + lane) * 16);
-                            for (int j = 0; j < 4; ++j) {
-                                x[2 * j] = from_half(v[j] & 0xFFFF);
-                                x[2 * j + 1] = from_half(v[j] >> 16);
-                            }
-                        }
-                        if (live) store8(out, y.type, wide, 32 * b + 8 * g, x);
+                    if constexpr (Q4) {
+                        load_words<GS>(tile + (m * 64 + lane) * GS * 4, k[m][0]);
+                        for (int e = 0; e < GS; ++e) ks[m * GS + e] = *reinterpret_cast<const uint16_t*>(tile + scale_offset(NB, false, i, m * GS + e));
+                    } else {
+                        for (int e = 0; e < GS; ++e) load_words<4>(tile + ((m * GS + e) * 64 + lane) * 16, k[m][e]);
                     }
                 }
-                continue;
             }
-            const uint8_t* from = tile + tile_values_at(Q4, NB);
+            if (a.v.data != nullptr) {
 #pragma unroll
-            for (int m = 0; m < NG; ++m) {
-                uint32_t w[Q4 ? 1 : 4][GS], d[Q4 ? 2 * GS : 1];
-                if constexpr (Q4) {
-                    load_words<GS>(from + (m * 64 + lane) * GS * 4, w[0]);
-                    load_words<2 * GS>(tile + tile_value_scales_at(NB) + (g * NB + m * GS) * 8, d);
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) load_words<GS>(from + ((r * NG + m) * 64 + lane) * GS * 4, w[r]);
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int32_t row = row0 + 4 * g + r;
-                    if (row < sr.begin || row >= sr.end) continue;
-                    char* out = row_ptr(y, row, h);
-#pragma unroll
-                    for (int e = 0; e < GS; ++e) {
-                        float x[2];
-                        if constexpr (Q4) {
-                            const uint32_t c = w[0][e] >> ((r & 1) * 16 + (r >> 1) * 8);
-                            const float f = from_half(d[2 * e + r / 2] >> (r % 2 * 16) & 0xFFFF);
-                            x[0] = (static_cast<float>(c & 15) - 8) * f;
-                            x[1] = (static_cast<float>(c >> 4 & 15) - 8) * f;
-                        } else {
-                            x[0] = from_half(w[r][e] & 0xFFFF);
-                            x[1] = from_half(w[r][e] >> 16);
-                        }
-                        store2(out, y.type, wide, 32 * (m * GS + e) + 2 * i, x);
+                for (int m = 0; m < NG; ++m) {
+                    if constexpr (Q4) {
+                        load_words<GS>(from + (m * 64 + lane) * GS * 4, v[m][0]);
+                        load_words<2 * GS>(tile + tile_value_scales_at(NB) + (g * NB + m * GS) * 8, vs[m]);
+                    } else {
+                        for (int r = 0; r < 4; ++r) load_words<GS>(from + ((r * NG + m) * 64 + lane) * GS * 4, v[m][r]);
                     }
+                }
+            }
+            const int32_t row0 = sr.begin + (t0 - sr.first);  // of the tile's first position; rows before sr.begin are not there
+            const auto to = [&](int32_t row, const HeadRows& y) -> char* { return row >= sr.begin && row < sr.end ? row_ptr(y, row, h) : nullptr; };
+            if (a.k.data != nullptr) {
+                char* out = to(row0 + i, a.k);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float x[8];
+                    if constexpr (Q4) key_codes(k[b / GS][0][b % GS], from_half(ks[b]), x);
+                    else halves8(k[b / GS][b % GS], x);
+                    if (out != nullptr) store8<true>(out, a.k.type, vec & 1, 32 * b + 8 * g, x);
+                }
+            }
+            if (a.v.data != nullptr) {
+                char* out = to(row0 + 4 * g + i % 4, a.v);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const int m = b / GS, e = b % GS;
+                    float x[8];
+                    if constexpr (Q4) {
+                        const uint32_t c = untransposed(v[m][0][e], lane);
+                        const float d = from_half(vs[m][2 * e + i % 4 / 2] >> (i % 2 * 16) & 0xFFFF);
+                        for (int j = 0; j < 8; ++j) x[j] = (static_cast<float>(c >> (4 * j) & 15) - 8) * d;
+                    } else {
+                        uint32_t t[4] = {v[m][0][e], v[m][1][e], v[m][2][e], v[m][3][e]};
+                        transpose_words(t, lane);
+                        halves8(t, x);
+                    }
+                    if (out != nullptr) store8<true>(out, a.v.type, vec & 2, 32 * b + i / 4 * 8, x);
                 }
             }
         }
@@ -560,7 +569,7 @@ hipError_t launch_kv_append(const AppendArgs& a, hipStream_t st) {
 
 hipError_t launch_kv_read(const ReadArgs& a, hipStream_t st) {
     const int vec = (a.k.data != nullptr && wide(a.k) ? 1 : 0) | (a.v.data != nullptr && wide(a.v) ? 2 : 0);
-    const dim3 grid = tile_grid(a.b, static_cast<uint64_t>(a.kv.kv_heads) * (a.k.data != nullptr && a.v.data != nullptr ? 2 : 1));
+    const dim3 grid = tile_grid(a.b, a.kv.kv_heads);
     switch (a.kv.head_dim / 32) {
         case 2: return launch_read<2>(a, grid, vec, st);
         case 3: return launch_read<3>(a, grid, vec, st);

@@ -83,12 +83,20 @@ __device__ inline void load8(const void* head, int type, bool vec, int d, float 
     }
 }
 
+// PAST: past the caches, for rows that are written in pieces and not read again soon.
+template <bool PAST, typename T>
+__device__ inline void store(T* p, T x) {
+    if constexpr (PAST) __builtin_nontemporal_store(x, p);
+    else *p = x;
+}
+
+template <bool PAST = false>
 __device__ inline void store8(void* head, int type, bool vec, int d, const float (&x)[8]) {
     if (type == kTypeF32) {
         float* p = static_cast<float*>(head) + d;
         if (vec) {
-            *reinterpret_cast<float4v*>(p) = float4v{x[0], x[1], x[2], x[3]};
-            *reinterpret_cast<float4v*>(p + 4) = float4v{x[4], x[5], x[6], x[7]};
+            store<PAST>(reinterpret_cast<float4v*>(p), float4v{x[0], x[1], x[2], x[3]});
+            store<PAST>(reinterpret_cast<float4v*>(p + 4), float4v{x[4], x[5], x[6], x[7]});
         } else {
             for (int j = 0; j < 8; ++j) p[j] = x[j];
         }
@@ -98,7 +106,7 @@ __device__ inline void store8(void* head, int type, bool vec, int d, const float
     for (int j = 0; j < 8; ++j) u[j] = type == kTypeF16 ? to_half(x[j]) : to_bf16(x[j]);
     uint16_t* p = static_cast<uint16_t*>(head) + d;
     if (vec) {
-        *reinterpret_cast<word4v*>(p) = word4v{u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16};
+        store<PAST>(reinterpret_cast<word4v*>(p), word4v{u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16});
     } else {
         for (int j = 0; j < 8; ++j) p[j] = static_cast<uint16_t>(u[j]);
     }
@@ -183,24 +191,11 @@ __device__ inline void store_words(uint8_t* p, const uint32_t (&w)[N]) {
     *reinterpret_cast<Words<N, ALIGN>*>(p) = x;
 }
 
-__device__ inline void store2(void* head, int type, bool vec, int d, const float (&x)[2]) {
-    if (type == kTypeF32) {
-        float* p = static_cast<float*>(head) + d;
-        if (vec) {
-            *reinterpret_cast<word2v*>(p) = word2v{__builtin_bit_cast(uint32_t, x[0]), __builtin_bit_cast(uint32_t, x[1])};
-        } else {
-            p[0] = x[0];
-            p[1] = x[1];
-        }
-        return;
-    }
-    const uint32_t lo = type == kTypeF16 ? to_half(x[0]) : to_bf16(x[0]), hi = type == kTypeF16 ? to_half(x[1]) : to_bf16(x[1]);
-    uint16_t* p = static_cast<uint16_t*>(head) + d;
-    if (vec) {
-        *reinterpret_cast<uint32_t*>(p) = lo | hi << 16;
-    } else {
-        p[0] = static_cast<uint16_t>(lo);
-        p[1] = static_cast<uint16_t>(hi);
+// Eight halves.
+__device__ inline void halves8(const uint32_t (&w)[4], float (&x)[8]) {
+    for (int j = 0; j < 4; ++j) {
+        x[2 * j] = from_half(w[j] & 0xFFFF);
+        x[2 * j + 1] = from_half(w[j] >> 16);
     }
 }
 
