@@ -3,8 +3,8 @@
 // As in paged_attention.hip the product's sides are swapped, S^T = K Q^T and O^T = V^T P^T, here with
 // v_mfma_f32_32x32x16_f16 (twice the rate of the 16-wide one: 2.08 against 1.14 PFLOP/s measured), and
 // a lane's probabilities are its second product's operand as they stand.  Keys and values pass through
-// LDS, 64 positions at a time, as halves in operand order: a tile is unpacked once for the workgroup's
-// columns, and an operand is one conflict-free 16-byte read of a lane.
+// LDS, 64 or 128 positions at a time, as halves in operand order: a tile is unpacked once for the workgroup's
+// columns, and an operand is one conflict-free 16-byte read of a lane.  (128 in the place of 64: 263 us for 306, half the barriers.)
 #include <algorithm>
 
 #include "paged.h"
@@ -129,9 +129,17 @@ __device__ inline void unpack(const RawTile<NB, Q4>& raw, BlockLds<NB, PLANES, S
     }
 }
 
-// A workgroup takes 256 columns and one part of the positions, a wave 32 columns.  Without a window half of the
+// A workgroup takes 256 columns, or 128, and one part of the positions, a wave 32 columns.  Without a window half of eight
 // waves' columns are from the front of the prompt and half are their mirror image from the back: what
-// two such waves, which share a SIMD, see adds up to the same for all.
+// two such waves, which share a SIMD, see adds up to the same for all.  Four waves have a SIMD each and columns next to each
+// other, the last of the prompt, which see most, first.
+//
+// Bound by the issue of vector and matrix instructions together.  4000 rows of 8100 positions, 16 heads of 128 in 4 bits: 263 us,
+// 760 TFLOP/s, where the products and their operands' reads take 160, the softmax 30, the unpacking 45 and the fetches and
+// searches for what is not finite the rest, as far as they do not overlap; of fp16 pages 304.  With four waves, one a SIMD, the latter
+// take 443: a lone wave issues a vector instruction every eight cycles, two every four each.  Heads of 256 do not
+// fit eight: 494 us spilled, 137 by four (2000 rows of 4000, 8 heads in 4 bits; 360 TFLOP/s).  Four for 32-bit results: 406 spilled, 236 (2000 of
+// 4000, 16 heads of 128 in 4 bits, three products in the place of one).
 template <int NB, bool Q4, bool EXACT>
 __global__ __launch_bounds__(64 * waves_of(NB, EXACT)) __attribute__((amdgpu_waves_per_eu(waves_of(NB, EXACT) / 4, waves_of(NB, EXACT) / 4))) void k_paged_prompt(PagedAttnArgs a) {
     constexpr int HD = 32 * NB, PLANES = Q4 && EXACT ? 2 : 1, PARTS = EXACT ? 2 : 1, PRODUCTS = EXACT + PLANES, kWaves = waves_of(NB, EXACT);
@@ -157,7 +165,8 @@ __global__ __launch_bounds__(64 * waves_of(NB, EXACT)) __attribute__((amdgpu_wav
     for (uint32_t s = blockIdx.z; s < a.b.seqs; s += gridDim.z) {
         const SeqRows sr = seq_rows(a.b, s);
         const uint32_t cols = (sr.end - sr.begin) * a.group.d, tiles = (cols + kWide - 1) / kWide;
-        const uint32_t fronts = window == 0 ? (tiles + 1) / 2 : tiles, per_set = window == 0 ? kWaves / 2 : kWaves;
+        const bool mirrored = kWaves == 8 && window == 0;
+        const uint32_t fronts = mirrored ? (tiles + 1) / 2 : tiles, per_set = mirrored ? kWaves / 2 : kWaves, sets = (fronts + per_set - 1) / per_set;
         // the positions of a column tile's rows, and those that they see
         const auto range = [&](uint32_t t, int32_t& plo, int32_t& phi, int32_t& tlo, int32_t& thi) {
             const uint32_t last = std::min<uint32_t>((t + 1) * kWide, cols) - 1;
@@ -166,17 +175,17 @@ __global__ __launch_bounds__(64 * waves_of(NB, EXACT)) __attribute__((amdgpu_wav
             tlo = window != 0 && plo - window + 1 > 0 ? plo - window + 1 : 0;
             thi = std::min(phi + 1, capacity);
         };
-        for (uint32_t set = first_set; set * per_set < fronts; set += set_step) {
-            const uint32_t front = set * per_set, back_last = std::min(front + per_set, fronts) - 1;
+        for (uint32_t set = first_set; set < sets; set += set_step) {
+            const uint32_t front = (mirrored ? set : sets - 1 - set) * per_set, back_last = std::min(front + per_set, fronts) - 1;
             uint32_t tile = front + (wave & (per_set - 1));
-            if (window == 0 && wave >= kWaves / 2) tile = tile < fronts && tiles - 1 - tile >= fronts ? tiles - 1 - tile : tiles;
+            if (mirrored && wave >= kWaves / 2) tile = tile < fronts && tiles - 1 - tile >= fronts ? tiles - 1 - tile : tiles;
             else if (tile >= fronts) tile = tiles;
             int32_t pos_lo = 0, pos_hi = 0, t_lo = 0, t_hi = 0;
             if (tile < tiles) range(tile, pos_lo, pos_hi, t_lo, t_hi);
             const int32_t pos = tile * kWide + col < cols ? sr.first + static_cast<int32_t>(over(tile * kWide + col, a.group)) : pos_lo;
             int32_t wg_lo, wg_plo, wg_phi, wg_hi, y0, y1, y2;  // the workgroup's, from its first tile's to its last one's
             range(front, wg_plo, y0, wg_lo, y1);
-            range(window == 0 ? tiles - 1 - front : back_last, y0, wg_phi, y2, wg_hi);
+            range(mirrored ? tiles - 1 - front : back_last, y0, wg_phi, y2, wg_hi);
             const int32_t blk_lo = wg_lo / BLOCK, blocks = wg_hi > wg_lo ? (wg_hi + BLOCK - 1) / BLOCK - blk_lo : 0;
             const int32_t per = (blocks + static_cast<int32_t>(a.splits) - 1) / static_cast<int32_t>(a.splits);
             const int32_t blk_begin = blk_lo + static_cast<int32_t>(std::min<int64_t>(blocks, static_cast<int64_t>(per) * split));
