@@ -326,9 +326,12 @@ size_t brisk_hip_paged_attention_bytes(const brisk_hip_kv* kv, const brisk_hip_b
  * + 1) .. p (window 0: from 0), query head h reads key/value head
  * h / (heads / kv_heads), and out = sum softmax(scale q k) v.  What a row does not see has no part
  * in it, infinities and NaN included; a row that sees nothing, or only scores of
- * minus infinity, gives zeros.  q, out: [rows][heads][head_dim]; with 16-bit
- * queries and outputs, queries and probabilities are multiplied in 16 bits and
- * summed in 32; with F32 queries or outputs the products are those of 32 bits.
+ * minus infinity, gives zeros.  q, out: [rows][heads][head_dim], and out may be
+ * q (the same data, type and strides); with 16-bit queries and outputs,
+ * queries, probabilities and 4-bit values (in large prompts 4-bit keys too) are
+ * multiplied as 16-bit numbers and summed in 32 bits; with F32 queries or outputs the
+ * products are those of 32 bits.  The kernel is chosen for the whole batch: tokens
+ * beside long prompts are attended faster in a call of their own.
  * `workspace`: brisk_hip_paged_attention_bytes() bytes at least, 16-byte
  * aligned, used by this call alone while it runs (NULL where 0 are needed). */
 int brisk_hip_paged_attention(const brisk_hip_kv* kv, const brisk_hip_batch* batch, const brisk_hip_heads* q, uint32_t heads,

@@ -547,6 +547,48 @@ def test_attention_shared_pages_and_repeats(lib):
         assert torch.equal(out, cache.attend(q, 0.125))
 
 
+@pytest.mark.usefixtures("tables")
+@pytest.mark.parametrize("src", [F16, F32], ids=NAMES.get)
+@pytest.mark.parametrize("rows_", [[1, 3], [300, 130]], ids=["few", "many"])
+def test_attention_into_its_queries(lib, src, rows_):
+    """The output in the queries' place: the same bits as beside them."""
+    batch = Batch(rows_, [900, 333], 32)
+    cache = filled(lib, batch, Q4_0, 2, 128)
+    q = rows(np.random.default_rng(5), batch.n, 8, 128, src).cuda()
+    want = cache.attend(q, 0.09)
+    cache.attend(q, 0.09, out=q)
+    assert torch.equal(q, want)
+
+
+@pytest.mark.usefixtures("tables")
+@pytest.mark.parametrize("kind,src,heads,kvh,dim", [(Q4_0, F16, 4, 1, 256), (F16, F32, 4, 2, 64), (Q4_0, BF16, 6, 3, 128)])
+def test_attention_of_prompts_captured(lib, kind, src, heads, kvh, dim):
+    """A prompt's call captured, and replayed over lengths and tables that changed, with eager calls between: the eager call's bits."""
+    batches = [Batch([200, 90], lengths, 16, seed=n, pool=120) for n, lengths in enumerate([[700, 333], [200, 700], [411, 90]])]
+    widest = max(b.stride for b in batches)
+    for b in batches:
+        b.table, b.stride = np.pad(b.table, ((0, 0), (0, widest - b.stride)), constant_values=-1), widest
+    cache = Cache(lib, batches[0], kind, kvh, dim, max_rows=200, max_length=700)
+    cache.memory.view(torch.float16).copy_(torch.rand(cache.memory.numel() // 2, device="cuda").half())
+    q = rows(np.random.default_rng(5), 290, heads, dim, src).cuda()
+    out, work = torch.zeros_like(q), cache.workspace(heads)
+    cache.attend(q, 0.09, out=out, work=work)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        cache.attend(q, 0.09, out=out, work=work)
+    held = cache.arrays
+    for b in batches + batches[::-1]:
+        cache.set(b)
+        want = cache.attend(q, 0.09)
+        for mine, new in zip(held, cache.arrays):
+            mine.copy_(new)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 # ---------------------------------------------------------------- together, as a program uses them
 
 @pytest.mark.parametrize("kind", [F16, Q4_0], ids=NAMES.get)
