@@ -273,13 +273,19 @@ __device__ inline uint32_t transposed(uint32_t w, int lane) {
     return __builtin_amdgcn_perm(b, w, lane & 2 ? 0x03070206 : 0x05010400);
 }
 
+// Where a rotation's pairs are: adjacent, whole blocks apart, or anywhere.
+constexpr int kAdjacent = 0, kBlocks = 1, kFar = 2;
+
 // One wave a tile's keys or values: lane 16 g + i has dimensions 32 b + 8 g + 0..7 of position i, for each block b, which is
-// how the tile holds keys.  A rotation's pairs lie in one lane (adjacent, or half the rotated dimensions,
-// whole blocks, apart); norms and quantisation cross four lanes, 4-bit values' bytes four others.
-// Bound by memory in long prompts; rows of single tokens use one lane in 16, and cost a launch.
-template <int NB, bool Q4>
+// how the tile holds keys.  A rotation's pairs lie in one lane where they are adjacent or half the rotated dimensions,
+// whole blocks, apart; norms and quantisation cross four lanes, 4-bit values' bytes four others.
+// Bound by the latency of what a wave reads: 8190 rows of 8 heads of 64, f32 to 4 bits, take 17 us (3.3 TB/s; 11 at a copy's rate), a call of
+// 8000 of 8 heads of 128 with norms, bf16 to fp16, 39 (all reads at once; 46 one after the other), and 48 single tokens, one
+// lane in 16, 8, of which a launch is 4.
+template <int NB, bool Q4, int PAIRS>
 __global__ __launch_bounds__(kThreads) void k_kv_append_tiles(AppendArgs a) {
     constexpr int GS = NB < 4 ? NB : 4, NG = NB / GS, HD = 32 * NB;
+    constexpr bool IN_LANE = PAIRS != kFar, NEOX = PAIRS == kBlocks, EARLY = NB <= 8 && IN_LANE;  // (the others have no registers for early loads)
     const int lane = static_cast<int>(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = lane % 16, g = lane / 16;
     for (uint32_t s = blockIdx.y; s < a.b.seqs; s += gridDim.y) {
         const SeqRows sr = seq_rows(a.b, s);
@@ -291,67 +297,109 @@ __global__ __launch_bounds__(kThreads) void k_kv_append_tiles(AppendArgs a) {
             const bool value = rest >= a.kv.kv_heads;
             const uint32_t h = value ? rest - a.kv.kv_heads : rest;
             const int32_t t0 = (t_lo + static_cast<int32_t>(n)) * 16, page = page_of(a.kv, a.b, s, t0), pos = t0 + i;
-            if (page < 0) continue;
             const int32_t row = sr.begin + (pos - sr.first);
             const bool live = row >= sr.begin && row < sr.end && (a.rope.table == nullptr || static_cast<uint32_t>(pos) < a.rope.positions);
             const bool full = __all(live);
             if (!__any(live)) continue;
-            uint8_t* tile = a.kv.data + tile_at(a.kv, page, h, t0);
             const HeadRows& from = value ? a.v : a.k;
             const char* head = row_ptr(from, live ? row : sr.begin, h);
+            // all that is read is on its way at once: rows, norm weights and the rotation's (cos, sin)
             float y[NB][8];
 #pragma unroll
             for (int b = 0; b < NB; ++b) load8(head, from.type, true, 32 * b + 8 * g, y[b]);
-            if (!value && (a.w != nullptr || a.rope.table != nullptr)) {
-                double x[NB][8], scale = 1;
+            const int dims = static_cast<int>(a.rope.dims);
+            const float* cs = !value && a.rope.table != nullptr ? a.rope.table + static_cast<size_t>(live ? pos : 0) * a.rope.dims : nullptr;
+            float t[EARLY ? NB : 1][8], wt[EARLY ? NB : 1][8];
+            if (EARLY && !value && a.w != nullptr) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    for (int j = 0; j < 8; ++j) wt[EARLY ? b : 0][j] = a.w[32 * b + 8 * g + j];
+            }
+            if (EARLY && cs != nullptr && IN_LANE) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    // (half a head's blocks of pairs take two blocks of the table each)
+                    const int d = NEOX ? b / 2 * 64 + 16 * g + b % 2 * 8 : 32 * b + 8 * g;
+                    if (d < dims) load8(cs, kTypeF32, true, d, t[EARLY ? b : 0]);
+                }
+            }
+            if (page < 0) continue;
+            uint8_t* tile = a.kv.data + tile_at(a.kv, page, h, t0);
+            if (!value && (a.w != nullptr || cs != nullptr)) {
+                double scale = 1;
                 if (a.w != nullptr) {
-                    double sum = 0;
+                    double sums[4] = {};
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
-                        for (int j = 0; j < 8; ++j) sum = __builtin_fma(static_cast<double>(y[b][j]), static_cast<double>(y[b][j]), sum);
+                        for (int j = 0; j < 8; ++j) sums[j % 4] = __builtin_fma(static_cast<double>(y[b][j]), static_cast<double>(y[b][j]), sums[j % 4]);
+                    double sum = sums[0] + sums[1] + (sums[2] + sums[3]);
                     sum += __shfl_xor(sum, 16);
                     sum += __shfl_xor(sum, 32);
                     scale = 1.0 / sqrt(sum / HD + static_cast<double>(a.eps));
                 }
+                const auto weighed = [&](float z, float w) { return a.w != nullptr ? static_cast<double>(z) * scale * static_cast<double>(w) : static_cast<double>(z); };
+                const auto weight_of = [&](int b, int j) { return EARLY ? wt[EARLY ? b : 0][j] : a.w != nullptr ? a.w[32 * b + 8 * g + j] : 0.0f; };
+                const auto plain = [&](int b) {
+                    for (int j = 0; j < 8; ++j) y[b][j] = static_cast<float>(weighed(y[b][j], weight_of(b, j)));
+                };
+                bool turned[NB] = {};  // (of blocks: known where a block's number is)
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    for (int j = 0; j < 8; ++j) {
-                        x[b][j] = y[b][j];
-                        if (a.w != nullptr) x[b][j] = x[b][j] * scale * static_cast<double>(a.w[32 * b + 8 * g + j]);
-                        y[b][j] = static_cast<float>(x[b][j]);
-                    }
-                }
-                if (a.rope.table != nullptr) {
-                    const float* cs = a.rope.table + static_cast<size_t>(live ? pos : 0) * a.rope.dims;
-                    const int dims = static_cast<int>(a.rope.dims);
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const int d = 32 * b + 8 * g;
-                        if (!a.rope.neox) {
-                            if (d >= dims) continue;
-                            float t[8];
-                            load8(cs, kTypeF32, true, d, t);
-#pragma unroll
-                            for (int j = 0; j < 8; j += 2) {
-                                y[b][j] = static_cast<float>(mul_sub(x[b][j], static_cast<double>(t[j]), x[b][j + 1], static_cast<double>(t[j + 1])));
-                                y[b][j + 1] = static_cast<float>(mul_add(x[b][j], static_cast<double>(t[j + 1]), x[b][j + 1], static_cast<double>(t[j])));
-                            }
+                    int d = 32 * b + 8 * g;
+                    if constexpr (!IN_LANE) asm volatile("" : "+v"(d));  // (or the places of all of a head's partners are held in registers)
+                    if (NEOX ? turned[b] : false) continue;
+                    if (cs == nullptr || (IN_LANE ? !NEOX && d >= dims : 32 * b >= dims)) {
+                        plain(b);
+                    } else if constexpr (!IN_LANE) {
+                        // pairs half the rotated dimensions apart, which another lane has: from the row once more; dimensions
+                        // that are not rotated (in this block, of other lanes) go the same way, and are chosen at the end
+                        const int half = dims / 2;
+                        const bool whole = half % 8 == 0;  // then the partners are eight in a row
+                        float other[8];
+                        if (whole) {
+                            load8(head, from.type, true, d >= dims ? d : d < half ? d + half : d - half, other);
                         } else {
-                            // dims / 64 blocks on: one of the lane's own, known when its number is
 #pragma unroll
-                            for (int o = 2 * b + 1; o < NB; ++o) {
-                                if (dims != 64 * (o - b)) continue;
-                                float t[16];
-                                load8(cs, kTypeF32, true, 2 * d, reinterpret_cast<float(&)[8]>(t[0]));
-                                load8(cs, kTypeF32, true, 2 * d + 8, reinterpret_cast<float(&)[8]>(t[8]));
+                            for (int j = 0; j < 8; ++j) other[j] = load1(head, from.type, d + j >= dims ? d + j : d + j < half ? d + j + half : d + j - half);
+                        }
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    const double c = t[2 * j], si = t[2 * j + 1];
-                                    y[b][j] = static_cast<float>(mul_sub(x[b][j], c, x[o][j], si));
-                                    y[o][j] = static_cast<float>(mul_add(x[b][j], si, x[o][j], c));
-                                }
+                        for (int j = 0; j < 8; ++j) {
+                            const int i = d + j, p = i >= dims ? i : i < half ? i + half : i - half, e = i >= dims ? 0 : i < half ? i : i - half;
+                            const double x = weighed(y[b][j], weight_of(b, j)), z = weighed(other[j], a.w != nullptr ? a.w[p] : 0.0f), c = cs[2 * e], si = cs[2 * e + 1];
+                            const double r = i < half ? mul_sub(x, c, z, si) : mul_add(z, si, x, c);
+                            y[b][j] = static_cast<float>(i < dims ? r : x);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);  // (a block's loads at a time)
+                    } else if constexpr (!NEOX) {
+                        float u[8];
+                        if constexpr (!EARLY) load8(cs, kTypeF32, true, d, u);
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2) {
+                            const double x = weighed(y[b][j], weight_of(b, j)), z = weighed(y[b][j + 1], weight_of(b, j + 1));
+                            const double c = EARLY ? t[EARLY ? b : 0][j] : u[j], si = EARLY ? t[EARLY ? b : 0][j + 1] : u[j + 1];
+                            y[b][j] = static_cast<float>(mul_sub(x, c, z, si));
+                            y[b][j + 1] = static_cast<float>(mul_add(x, si, z, c));
+                        }
+                    } else {
+                        // dims / 64 blocks on: one of the lane's own, known when its number is
+#pragma unroll
+                        for (int o = 2 * b + 1; o < NB; ++o) {
+                            if (dims != 64 * (o - b)) continue;
+                            turned[b] = turned[o] = true;
+                            float u[16];
+                            if constexpr (!EARLY) {
+                                load8(cs, kTypeF32, true, 2 * d, reinterpret_cast<float(&)[8]>(u[0]));
+                                load8(cs, kTypeF32, true, 2 * d + 8, reinterpret_cast<float(&)[8]>(u[8]));
+                            }
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const double c = EARLY ? t[EARLY ? 2 * b + j / 4 : 0][2 * j % 8] : u[2 * j], si = EARLY ? t[EARLY ? 2 * b + j / 4 : 0][2 * j % 8 + 1] : u[2 * j + 1];
+                                const double x = weighed(y[b][j], weight_of(b, j)), z = weighed(y[o][j], weight_of(o, j));
+                                y[b][j] = static_cast<float>(mul_sub(x, c, z, si));
+                                y[o][j] = static_cast<float>(mul_add(x, si, z, c));
                             }
                         }
+                        if (!turned[b]) plain(b);
                     }
                 }
             }
@@ -409,11 +457,18 @@ __global__ __launch_bounds__(kThreads) void k_kv_append_tiles(AppendArgs a) {
     }
 }
 
+template <int NB, int PAIRS>
+hipError_t launch_append_pairs(const AppendArgs& a, dim3 grid, hipStream_t st) {
+    if (a.kv.q4) k_kv_append_tiles<NB, true, PAIRS><<<grid, dim3(kThreads), 0, st>>>(a);
+    else k_kv_append_tiles<NB, false, PAIRS><<<grid, dim3(kThreads), 0, st>>>(a);
+    return hipGetLastError();
+}
 template <int NB>
 hipError_t launch_append(const AppendArgs& a, dim3 grid, hipStream_t st) {
-    if (a.kv.q4) k_kv_append_tiles<NB, true><<<grid, dim3(kThreads), 0, st>>>(a);
-    else k_kv_append_tiles<NB, false><<<grid, dim3(kThreads), 0, st>>>(a);
-    return hipGetLastError();
+    if (a.rope.table == nullptr || !a.rope.neox) return launch_append_pairs<NB, kAdjacent>(a, grid, st);
+    if (a.rope.dims % 64 == 0) return launch_append_pairs<NB, kBlocks>(a, grid, st);
+    if constexpr (NB <= 4) return launch_append_pairs<NB, kFar>(a, grid, st);
+    return hipErrorInvalidValue;
 }
 
 // The inverse of transposed(): a word's positions in the order 0, 2, 1, 3 go to the four lanes, in the order of the dimensions.
@@ -549,9 +604,11 @@ hipError_t launch_norm_rope(const NormRopeArgs& a, hipStream_t st) {
 }
 
 hipError_t launch_kv_append(const AppendArgs& a, hipStream_t st) {
-    // By tiles where rows are read 16 bytes at a time and a rotation's pairs lie in one lane; otherwise row by row.
-    const bool turned_in_lane = a.rope.table == nullptr || (reinterpret_cast<uintptr_t>(a.rope.table) % 16 == 0 && a.rope.dims % (a.rope.neox ? 64 : 8) == 0);
-    if (wide(a.k) && wide(a.v) && turned_in_lane) {
+    // By tiles where rows and the table are read 16 bytes at a time, and registers hold a rotation across lanes; otherwise row by row
+    // (2653 rows of three sequences, 16 heads of 96 in 4 bits, 24 dimensions rotated: 160 us so, and 75 by tiles).
+    const bool far = a.rope.table != nullptr && a.rope.neox && a.rope.dims % 64 != 0;
+    const bool wide_table = a.rope.table == nullptr || (reinterpret_cast<uintptr_t>(a.rope.table) % 16 == 0 && a.rope.dims % 8 == 0);
+    if (wide(a.k) && wide(a.v) && (far ? a.kv.head_dim <= 128 : wide_table)) {
         const dim3 grid = tile_grid(a.b, a.pairs.d);
         switch (a.kv.head_dim / 32) {
             case 2: return launch_append<2>(a, grid, st);

@@ -213,6 +213,15 @@ def test_append_and_read(lib, kind, dim, dims, neox, norm, src, page):
 
 
 @pytest.mark.parametrize("kind", [F16, Q4_0], ids=NAMES.get)
+@pytest.mark.parametrize("dim,dims,neox,norm,src", [(64, 16, 1, True, F32), (64, 20, 1, False, F16), (64, 2, 1, True, F32), (96, 24, 1, True, F16), (96, 96, 1, False, BF16), (128, 32, 1, True, BF16),
+                                                    (128, 100, 1, True, F32), (128, 112, 1, False, F32), (128, 64, 1, True, F16), (256, 128, 1, True, F32), (256, 96, 1, True, F16),
+                                                    (512, 256, 1, True, BF16), (512, 20, 1, False, F32), (128, 40, 2, True, F32), (96, 20, 2, False, F16), (256, 2, 2, True, F32)])
+def test_append_rotations(lib, kind, dim, dims, neox, norm, src):
+    """Pairs in a lane, in others, in other blocks; part of the head; tables whose rows are not 16-byte aligned."""
+    test_append_and_read(lib, kind, dim, dims, neox, norm, src, 32)
+
+
+@pytest.mark.parametrize("kind", [F16, Q4_0], ids=NAMES.get)
 def test_append_special_values(lib, kind):
     """Zero blocks, ties, equal magnitudes of either sign, subnormal scales, infinities, NaN, values past 16 bits."""
     rng = np.random.default_rng(5)
