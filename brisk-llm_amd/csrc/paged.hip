@@ -91,7 +91,8 @@ __device__ inline void turned(const void* head, int type, bool vec, int d, int h
     }
 }
 
-// One group of lanes a head.  A head's lanes read all they need before they write, so y may be x.
+// One group of lanes a head.  A head's lanes read all they need before they write, so y may be x.  Bound by memory: 4011 rows of 40 heads of 64,
+// f32 to bf16, 16.7 us, 3.8 TB/s; one row by its launch and one round trip, 6.
 __global__ __launch_bounds__(kThreads) void k_norm_rope(NormRopeArgs a, int lanes, int vec) {
     const int lane = static_cast<int>(threadIdx.x) % lanes, d = lane * 8;
     const uint32_t per = kThreads / lanes, total = static_cast<uint32_t>(a.n) * a.all.d;
