@@ -490,27 +490,28 @@ __device__ inline void transpose_words(uint32_t (&x)[4], int lane) {
     }
 }
 
-// One wave a tile: loads of the whole of it, as the attention's, keys' and values' on their way together.  A lane
-// then has eight values of a position, of values after a transposition among four lanes, and four lanes write 64 bytes or
-// more of a row, past the caches: 4 sequences of 16000 positions, 8 heads of 128 in 4 bits to fp16, take 56 us, as long as a
-// copy of as many bytes (5.2 TB/s), and through the caches 86.
+// One wave a tile's keys or values: loads of the whole of them, as the attention's.  A lane then has eight values of a position, of values after a transposition among four lanes, and four lanes write 64 bytes or
+// more of a row, past the caches: 4 sequences of 16000 positions, 8 heads of 128 in 4 bits to fp16, take 50 us, less than a
+// copy of as many bytes (5.8 TB/s), and through the caches 86.  (Keys and values by one wave: 8 us for 48 single rows in the place of 5.)
 template <int NB, bool Q4>
 __global__ __launch_bounds__(kThreads) void k_kv_read(ReadArgs a, int vec) {
     constexpr int GS = NB < 4 ? NB : 4, NG = NB / GS;
     const int lane = static_cast<int>(threadIdx.x) % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = lane % 16, g = lane / 16;
+    const uint32_t sides = a.k.data != nullptr && a.v.data != nullptr ? 2 : 1;
     for (uint32_t s = blockIdx.y; s < a.b.seqs; s += gridDim.y) {
         const SeqRows sr = seq_rows(a.b, s);
         if (sr.end <= sr.begin) continue;
         const int32_t last = sr.first + (sr.end - sr.begin) - 1, t_lo = sr.first < 0 ? 0 : sr.first / 16, t_hi = last < 0 ? 0 : last / 16 + 1;
-        const uint32_t total = (t_hi - t_lo) * a.heads.d;
-        for (uint32_t u = blockIdx.x * 4 + wave; u < total; u += gridDim.x * 4) {
-            const uint32_t n = over(u, a.heads), h = u - n * a.heads.d;
+        const uint32_t total = (t_hi - t_lo) * a.heads.d * sides;
+        for (uint32_t w = blockIdx.x * 4 + wave; w < total; w += gridDim.x * 4) {
+            const uint32_t u = w / sides, n = over(u, a.heads), h = u - n * a.heads.d;
+            const bool value = sides == 2 ? w % 2 != 0 : a.k.data == nullptr;
             const int32_t t0 = (t_lo + static_cast<int32_t>(n)) * 16, page = page_of(a.kv, a.b, s, t0);
             if (page < 0) continue;
             const uint8_t *tile = a.kv.data + tile_at(a.kv, page, h, t0), *from = tile + tile_values_at(Q4, NB);
             uint32_t k[NG][Q4 ? 1 : GS][Q4 ? GS : 4], v[NG][Q4 ? 1 : 4][GS], vs[NG][Q4 ? 2 * GS : 1];
             uint16_t ks[Q4 ? NB : 1];
-            if (a.k.data != nullptr) {
+            if (!value) {
 #pragma unroll
                 for (int m = 0; m < NG; ++m) {
                     if constexpr (Q4) {
@@ -521,7 +522,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_read(ReadArgs a, int vec) {
                     }
                 }
             }
-            if (a.v.data != nullptr) {
+            if (value) {
 #pragma unroll
                 for (int m = 0; m < NG; ++m) {
                     if constexpr (Q4) {
@@ -534,7 +535,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_read(ReadArgs a, int vec) {
             }
             const int32_t row0 = sr.begin + (t0 - sr.first);  // of the tile's first position; rows before sr.begin are not there
             const auto to = [&](int32_t row, const HeadRows& y) -> char* { return row >= sr.begin && row < sr.end ? row_ptr(y, row, h) : nullptr; };
-            if (a.k.data != nullptr) {
+            if (!value) {
                 char* out = to(row0 + i, a.k);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
@@ -544,7 +545,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_read(ReadArgs a, int vec) {
                     if (out != nullptr) store8<true>(out, a.k.type, vec & 1, 32 * b + 8 * g, x);
                 }
             }
-            if (a.v.data != nullptr) {
+            if (value) {
                 char* out = to(row0 + 4 * g + i % 4, a.v);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
@@ -627,7 +628,7 @@ hipError_t launch_kv_append(const AppendArgs& a, hipStream_t st) {
 
 hipError_t launch_kv_read(const ReadArgs& a, hipStream_t st) {
     const int vec = (a.k.data != nullptr && wide(a.k) ? 1 : 0) | (a.v.data != nullptr && wide(a.v) ? 2 : 0);
-    const dim3 grid = tile_grid(a.b, a.kv.kv_heads);
+    const dim3 grid = tile_grid(a.b, static_cast<uint64_t>(a.kv.kv_heads) * (a.k.data != nullptr && a.v.data != nullptr ? 2 : 1));
     switch (a.kv.head_dim / 32) {
         case 2: return launch_read<2>(a, grid, vec, st);
         case 3: return launch_read<3>(a, grid, vec, st);
