@@ -490,8 +490,9 @@ __device__ inline void transpose_words(uint32_t (&x)[4], int lane) {
     }
 }
 
-// One wave a tile's keys or values: loads of the whole of them, as the attention's.  A lane then has eight values of a position, of values after a transposition among four lanes, and four lanes write 64 bytes or
-// more of a row, past the caches: 4 sequences of 16000 positions, 8 heads of 128 in 4 bits to fp16, take 50 us, less than a
+// One wave a tile's keys or values: loads of the whole of them, as the attention's.  A lane then has eight values of a
+// position, of values after a transposition among four lanes, and four lanes write 64 bytes or more of a row,
+// past the caches: 4 sequences of 16000 positions, 8 heads of 128 in 4 bits to fp16, take 50 us, less than a
 // copy of as many bytes (5.8 TB/s), and through the caches 86.  (Keys and values by one wave: 8 us for 48 single rows in the place of 5.)
 template <int NB, bool Q4>
 __global__ __launch_bounds__(kThreads) void k_kv_read(ReadArgs a, int vec) {
