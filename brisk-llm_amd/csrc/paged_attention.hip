@@ -638,6 +638,9 @@ uint32_t paged_splits(const PagedKv& kv, const PagedBatch& b, uint32_t heads, bo
     // 4 heads of 256, 146 us for 256, and 2000 of 4000 146 for 138.
     const uint64_t cus = wide == 128 && window == 0 ? 512 : 256;
     const uint64_t wanted = prompt ? cus / blocks : std::max<uint64_t>(target / blocks, std::min<uint64_t>((most + 8191) / 8192, room));
+    // A few steps of a wave cost less than the join (a token of 16 heads of 128 at 333: 9.6 us a call in one part, 11.5 in three, at 500 10 and 11,
+    // at 1000 13 and 11; heads of 256 in 4 bits at 200 12 and 13, at 500 15.5 and 13.4).
+    if (!prompt && useful <= (kv.head_dim <= 128 ? 4 : 2)) return 1;
     return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(std::min(useful, wanted), kMaxSplits)));
 }
 
